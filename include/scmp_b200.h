@@ -289,6 +289,83 @@ int scmp_grouped_asymmetric_quant(const float* x, int rows, int cols, int group,
                                   float* scale_row, float* zp_row, float* x_int,
                                   float* group_stats, void* stream);
 
+/*
+ * The layers next to the SC matmul, exact (no counterpart in the reference,
+ * whose callers take them from their own model code): layer norm, the linear
+ * layer that a mixed-precision model keeps exact and that gives an SC layer its
+ * straight-through gradient, and 8-bit activation checkpoints for the backward
+ * pass. Tensors are float32, bfloat16 or float16 (enum scmp_dtype), row-major,
+ * with row pitches (ld*) counted in elements; statistics, sums and epilogues
+ * are float32 and rounded once on the way out. Results do not depend on timing
+ * (no atomic sums). Outputs are contiguous.
+ */
+enum scmp_dtype { SCMP_F32 = 0, SCMP_BF16 = 1, SCMP_F16 = 2 };
+enum scmp_activation {
+  SCMP_ACT_NONE = 0,
+  SCMP_ACT_RELU = 1,
+  SCMP_ACT_GELU = 2,      /* 0.5 v (1 + erf(v / sqrt 2))                         */
+  SCMP_ACT_GELU_TANH = 3, /* 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3)))     */
+  SCMP_ACT_SILU = 4       /* v / (1 + exp(-v))                                   */
+};
+
+/*
+ * 8-bit activation checkpoints: codes int8 (rows, cols) and exps uint8 (rows,
+ * ceil(cols/32)). Blocks of 32 values of a row share the power of two 2^e with
+ * e = floor(log2(max |x|)) - 6, at least -126 (float16: -24); a code is
+ * x * 2^-e rounded half to even, clamped to [-127, 127], and stands for
+ * code * 2^e, which every tensor type holds exactly. exps holds e + 127, or
+ * 255 for a block with an infinity or a NaN (it unpacks to NaN).
+ */
+int scmp_act8_pack(const void* x, int dtype, long long rows, int cols, long long ld, int8_t* codes,
+                   uint8_t* exps, void* stream);
+int scmp_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, int cols, void* out,
+                     int dtype, void* stream);
+
+/*
+ * Layer norm over rows of `cols`: y = (x - mean) * rstd * weight + bias with
+ * rstd = 1 / sqrt(mean((x - mean)^2) + eps). weight and bias may be NULL and
+ * are wdtype: float32 or x's type. mean and rstd (rows,) float32 may be NULL;
+ * codes and exps, when given, receive the 8-bit checkpoint of x.
+ * The backward pass takes x, or (x NULL) its checkpoint; dweight and dbias
+ * (wdtype) may be NULL, and need the workspace when they are not.
+ */
+int scmp_layer_norm_forward(const void* x, int dtype, long long rows, int cols, long long ldx,
+                            const void* weight, const void* bias, int wdtype, float eps, void* y,
+                            float* mean, float* rstd, int8_t* codes, uint8_t* exps, void* stream);
+int scmp_layer_norm_backward_workspace_size(long long rows, int cols, size_t* bytes);
+int scmp_layer_norm_backward(const void* dy, long long lddy, const void* x, long long ldx,
+                             const int8_t* codes, const uint8_t* exps, int dtype, long long rows,
+                             int cols, const float* mean, const float* rstd, const void* weight,
+                             int wdtype, void* dx, void* dweight, void* dbias, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Linear layer: pre = x weight^T + bias, y = act(pre) + residual, with
+ * x (rows, d), weight (m, d) as sc_matmul's operands a and b. bias (m,) is
+ * bias_dtype: float32 or x's type; bias and residual may be NULL. pre (rows, m)
+ * and its 8-bit checkpoint pre_codes, pre_exps are written where given.
+ */
+int scmp_linear_forward_workspace_size(int dtype, long long rows, int d, int m, size_t* bytes);
+int scmp_linear_forward(const void* x, long long ldx, const void* weight, long long ldw,
+                        const void* bias, int bias_dtype, const void* residual, long long ldr,
+                        int dtype, long long rows, int d, int m, int activation, void* y, void* pre,
+                        int8_t* pre_codes, uint8_t* pre_exps, void* workspace, size_t workspace_bytes,
+                        void* stream);
+/*
+ * Its gradients: dpre = dy * act'(pre), dx = dpre weight, dweight = dpre^T x,
+ * dbias = column sums of dpre (the residual's gradient is dy). Each of dx,
+ * dweight and dbias may be NULL. x (for dweight) and pre (for an activation)
+ * are given as tensors or as 8-bit checkpoints.
+ */
+int scmp_linear_backward_workspace_size(int dtype, long long rows, int d, int m, int activation,
+                                        int x_packed, int with_bias, size_t* bytes);
+int scmp_linear_backward(const void* dy, long long lddy, const void* x, long long ldx,
+                         const int8_t* x_codes, const uint8_t* x_exps, const void* weight,
+                         long long ldw, const void* pre, long long ldpre, const int8_t* pre_codes,
+                         const uint8_t* pre_exps, int dtype, long long rows, int d, int m,
+                         int activation, void* dx, void* dweight, void* dbias, int bias_dtype,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
 /* Profiling hook (no reference counterpart; the reference has no native
  * timing). While set, scmp_sc_matmul and scmp_enable_matmul record the CUDA
  * event gemm_start on their stream right before the SC-GEMM launch and

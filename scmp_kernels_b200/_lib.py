@@ -29,9 +29,12 @@ FLAG_NO_SPLIT = 0x2
 FLAG_B_READY = 0x4
 ABI_VERSION = 4
 MAX_OUT_PEERS = 8
+F32, BF16, F16 = 0, 1, 2
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 c_int, c_void_p, c_size_t, c_float, c_double = (ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t,
                                                 ctypes.c_float, ctypes.c_double)
+c_longlong = ctypes.c_longlong
 
 
 class MatmulDesc(ctypes.Structure):
@@ -96,6 +99,24 @@ SIGNATURES = {
                                              c_void_p, c_void_p, c_void_p, c_void_p]),
     "scmp_grouped_asymmetric_quant": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                               c_void_p, c_void_p, c_void_p, c_void_p]),
+    "scmp_act8_pack": (c_int, [c_void_p, c_int, c_longlong, c_int, c_longlong, c_void_p, c_void_p, c_void_p]),
+    "scmp_act8_unpack": (c_int, [c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p]),
+    "scmp_layer_norm_forward": (c_int, [c_void_p, c_int, c_longlong, c_int, c_longlong, c_void_p, c_void_p, c_int,
+                                        c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "scmp_layer_norm_backward_workspace_size": (c_int, [c_longlong, c_int, ctypes.POINTER(c_size_t)]),
+    "scmp_layer_norm_backward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int,
+                                         c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                         c_void_p, c_void_p, c_size_t, c_void_p]),
+    "scmp_linear_forward_workspace_size": (c_int, [c_int, c_longlong, c_int, c_int, ctypes.POINTER(c_size_t)]),
+    "scmp_linear_forward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_longlong,
+                                    c_int, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_size_t, c_void_p]),
+    "scmp_linear_backward_workspace_size": (c_int, [c_int, c_longlong, c_int, c_int, c_int, c_int, c_int,
+                                                    ctypes.POINTER(c_size_t)]),
+    "scmp_linear_backward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p,
+                                     c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int,
+                                     c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t,
+                                     c_void_p]),
 }
 
 _lib = None

@@ -10,14 +10,27 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
 OUT = os.path.join(HERE, "libscmp_b200.so")
-MAIN = os.path.join(HERE, "csrc", "scmp_b200.cu")
+OBJ_DIR = os.path.join(HERE, "_build")
+
+# Translation units and the sources each depends on (file names in csrc/; the
+# headers count for all).
+UNITS = {
+    "scmp_b200": ["scmp_b200.cu", "tables.cu", "quant.cu", "gemm_simt.cu", "gemm_tc.cu", "api.cu", "levels.cu",
+                  "quant_ref.cu", "noalloc.cu"],
+    "norms": ["norms.cu", "act8.cu", "layer_norm.cu"],
+    "linears": ["linears.cu", "linear_gemm.cu", "linear.cu"],
+}
+# Headers that only some units include.
+UNIT_HEADERS = {"internal.cuh": ("scmp_b200",), "quant.cuh": ("scmp_b200",), "vecio.cuh": ("norms", "linears"),
+                "act8.cuh": ("norms", "linears"), "linear.cuh": ("linears",)}
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-              "-Xcompiler", "-fPIC", "-shared", "-Xptxas", "-v"]
+              "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
 
 def _nvcc() -> str:
@@ -39,17 +52,41 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(s) <= t for s in sources())
 
 
+def _unit_sources(unit: str) -> list[str]:
+    csrc = os.path.join(HERE, "csrc")
+    headers = [h for h in sources() if h.endswith((".cuh", ".h"))
+               and unit in UNIT_HEADERS.get(os.path.basename(h), (unit,))]
+    return [os.path.join(csrc, f) for f in UNITS[unit]] + headers
+
+
+def _compile(unit: str, force: bool) -> str:
+    """Compile one unit when its object is older than its sources; the compiler's
+    report (ptxas registers, spills, shared memory per kernel) is kept beside it."""
+    obj = os.path.join(OBJ_DIR, unit + ".o")
+    srcs = _unit_sources(unit)
+    if not force and os.path.exists(obj) and all(os.path.getmtime(f) <= os.path.getmtime(obj) for f in srcs):
+        return ""
+    cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(REPO, "include"), "-c", "-o", obj, srcs[0]]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    with open(os.path.join(OBJ_DIR, unit + ".log"), "w") as f:
+        f.write(r.stdout + r.stderr)
+    if r.returncode:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"nvcc failed ({r.returncode}): {' '.join(cmd)}")
+    return r.stdout + r.stderr
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return OUT
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(REPO, "include"), "-o", OUT, MAIN]
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with ThreadPoolExecutor(len(UNITS)) as pool:  # the units compile side by side
+        reports = list(pool.map(lambda u: _compile(u, force), UNITS))
+    objs = [os.path.join(OBJ_DIR, u + ".o") for u in UNITS]
+    cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xcompiler", "-fPIC", "-o", OUT, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
-    # the compiler's report (ptxas registers, spills, shared memory per kernel)
-    os.makedirs(os.path.join(HERE, "_build"), exist_ok=True)
-    with open(os.path.join(HERE, "_build", "nvcc.log"), "w") as f:
-        f.write(r.stdout + r.stderr)
     if verbose or r.returncode:
-        sys.stderr.write(r.stdout + r.stderr)
+        sys.stderr.write("".join(reports) + r.stdout + r.stderr)
     if r.returncode:
         raise RuntimeError(f"nvcc failed ({r.returncode}): {' '.join(cmd)}")
     return OUT

@@ -1,0 +1,59 @@
+// 8-bit activation checkpoints: the number format.
+//
+// A row's values are kept in blocks of 32 (the last one shorter) that share a
+// power of two. With e = floor(log2(max |x|)) - 6, a value's code is
+// x * 2^-e rounded half to even and clamped to -127..127 (a block whose
+// largest value is above 127.5 / 128 of the next power of two saturates), and
+// stands for code * 2^e. e is kept as the byte e + 127, at least 1 (2^-126),
+// for float16 tensors at least 103 (2^-24, the type's smallest step). A block
+// that holds an infinity or a NaN has byte 255 and codes 0: it stands for NaN.
+//
+// Every step is exact but the one rounding to a code, so any two
+// implementations agree bit for bit; and a code has seven bits, so the value it
+// stands for is exact in bfloat16 and float16 (and so on the tensor cores),
+// which a free scale would not give. 1 + 1/32 bytes per value.
+#pragma once
+
+#include "vecio.cuh"
+
+namespace scmp {
+
+constexpr int kAct8Block = 32;
+constexpr uint32_t kAct8Nan = 255;
+
+__host__ __device__ constexpr int act8_blocks(int cols) { return (cols + kAct8Block - 1) / kAct8Block; }
+// Smallest exponent byte of a tensor type.
+template <class T>
+__host__ __device__ constexpr uint32_t act8_floor() { return Elem<T>::kDtype == SCMP_F16 ? 103u : 1u; }
+
+// Exponent byte of a block from the largest magnitude's bits (sign bit clear;
+// infinities and NaNs have exponent field 255 and compare above every number).
+__device__ __forceinline__ uint32_t act8_exponent(uint32_t top_bits, uint32_t floor_byte) {
+  const uint32_t ex = top_bits >> 23;
+  if (ex == 255u) return kAct8Nan;
+  return max((int)ex - 6, (int)floor_byte);
+}
+// 2^-e of an exponent byte (bytes 1..248 occur: normal floats).
+__device__ __forceinline__ float act8_inverse(uint32_t byte) {
+  return byte == kAct8Nan ? 0.f : __uint_as_float((254u - byte) << 23);
+}
+// 2^e; NaN for a block of non-finite values. A byte of 0 (never written by the
+// packers) stands for zero.
+__device__ __forceinline__ float act8_scale(uint32_t byte) {
+  return byte == kAct8Nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte << 23);
+}
+__device__ __forceinline__ int act8_code(float x, float inverse, bool nan_block) {
+  const int c = __float2int_rn(fclamp(fmul(x, inverse), -127.f, 127.f));
+  return nan_block ? 0 : c;
+}
+
+// The values of a checkpoint as a contiguous tensor of type dtype (act8.cu).
+cudaError_t launch_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, int cols, void* out, int dtype,
+                               cudaStream_t st);
+
+// out_k[c] = sum over p < parts of part[p][k][c], k < sets <= 2, in a fixed
+// order, as dtype; a null out is skipped (layer_norm.cu).
+cudaError_t launch_column_sum(const float* part, int parts, int sets, int cols, int dtype, void* out0, void* out1,
+                              cudaStream_t st);
+
+}  // namespace scmp

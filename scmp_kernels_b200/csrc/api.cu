@@ -5,10 +5,10 @@
 #include <string>
 
 #include "quant.cuh"
+#include "status.cuh"
 
 namespace scmp {
 
-static thread_local std::string t_last_error;
 static cudaEvent_t g_prof_start = nullptr, g_prof_stop = nullptr;
 static cudaEvent_t g_qprof_start = nullptr, g_qprof_stop = nullptr;
 
@@ -32,19 +32,6 @@ static cudaError_t launch_gemm(const GemmArgs& g, int flags, cudaStream_t st) {
   if (g_prof_stop) cudaEventRecord(g_prof_stop, st);
   return e;
 }
-
-static int fail(int code, const std::string& msg) {
-  t_last_error = msg;
-  return code;
-}
-static int cuda_fail(cudaError_t e, const char* what) {
-  return fail(SCMP_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-}
-#define SCMP_CUDA(call, what)                  \
-  do {                                         \
-    cudaError_t e_ = (call);                   \
-    if (e_ != cudaSuccess) return cuda_fail(e_, what); \
-  } while (0)
 
 // Bump allocator over the caller's workspace; a dry run only measures.
 struct Carver {
@@ -202,6 +189,9 @@ int scmp_device_error(int* code) {
   DeviceError h{0, 0}, z{0, 0};
   SCMP_CUDA(cudaMemcpyFromSymbol(&h, g_device_error, sizeof(h)), "scmp_device_error: read");
   SCMP_CUDA(cudaMemcpyToSymbol(g_device_error, &z, sizeof(z)), "scmp_device_error: clear");
+  DeviceError hl{0, 0};
+  SCMP_CUDA(linears_device_error(&hl), "scmp_device_error: read");
+  if (!h.code) h = hl;
   if (code) *code = h.code;
   if (h.code) {
     char buf[96];

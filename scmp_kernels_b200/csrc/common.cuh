@@ -58,8 +58,9 @@ struct DeviceError {
   int code;
   int where;
 };
-// Defined here: the library is a single translation unit (scmp_b200.cu).
-__device__ DeviceError g_device_error = {0, 0};
+// One record per translation unit (scmp_b200.cu, linears.cu);
+// scmp_device_error reads them all.
+static __device__ DeviceError g_device_error = {0, 0};
 
 __device__ __forceinline__ void record_error(int code, int where) {
   if (atomicCAS(&g_device_error.code, 0, code) == 0) g_device_error.where = where;

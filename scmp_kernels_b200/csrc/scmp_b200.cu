@@ -1,5 +1,6 @@
-// Single translation unit of libscmp_b200.so: the kernels share one device
-// error record, so they are compiled together instead of with -rdc.
+// Translation unit of the SC matmul: its kernels share one device error
+// record, so they are compiled together instead of with -rdc. The layers
+// around it are units of their own (norms.cu, linears.cu).
 #include "tables.cu"
 #include "quant.cu"
 #include "gemm_simt.cu"

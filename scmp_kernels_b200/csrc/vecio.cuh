@@ -1,0 +1,93 @@
+// Element types of the layers (float32, bfloat16, float16) and eight-value
+// loads and stores; all arithmetic is float32.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace scmp {
+
+template <class T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr int kDtype = SCMP_F32;
+  static __device__ __forceinline__ float to_f(float v) { return v; }
+  static __device__ __forceinline__ float from_f(float v) { return v; }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr int kDtype = SCMP_BF16;
+  static __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Elem<__half> {
+  static constexpr int kDtype = SCMP_F16;
+  static __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+};
+
+inline size_t dtype_size(int dtype) { return dtype == SCMP_F32 ? 4 : 2; }
+inline bool dtype_ok(int dtype) { return dtype == SCMP_F32 || dtype == SCMP_BF16 || dtype == SCMP_F16; }
+
+// Calls f with a null pointer of the element type (its type is what matters).
+template <class F>
+static auto with_dtype(int dtype, F&& f) {
+  if (dtype == SCMP_F32) return f((float*)nullptr);
+  if (dtype == SCMP_BF16) return f((__nv_bfloat16*)nullptr);
+  return f((__half*)nullptr);
+}
+
+// One value through the read-only path, as float32. 16-bit values are loaded as
+// integers: the 16-bit types' own __ldg is an asm statement without side
+// effects, which the compiler may run before the condition that guards it.
+template <class T>
+__device__ __forceinline__ float ldg1(const T* p) {
+  if constexpr (sizeof(T) == 2) {
+    const unsigned short u = __ldg(reinterpret_cast<const unsigned short*>(p));
+    return Elem<T>::to_f(*reinterpret_cast<const T*>(&u));
+  } else {
+    return __ldg(p);
+  }
+}
+
+// Eight consecutive values as they lie in memory (16 or 32 bytes, 16-byte aligned).
+template <class T>
+struct Raw8 {
+  uint4 q[sizeof(T) * 8 / 16];
+};
+template <class T>
+__device__ __forceinline__ Raw8<T> ldg8(const T* p) {
+  Raw8<T> r;
+  const uint4* s = reinterpret_cast<const uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) * 8 / 16); ++i) r.q[i] = __ldg(s + i);
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
+  const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f(e[i]);
+}
+template <class T>
+__device__ __forceinline__ void stg8(T* p, const float (&v)[8]) {
+  Raw8<T> r;
+  T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_f(v[i]);
+  uint4* d = reinterpret_cast<uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) * 8 / 16); ++i) d[i] = r.q[i];
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Rows of `cols` elements at a pitch of ld elements can be read 16 bytes at a time.
+inline bool rows_aligned16(const void* p, long long ld, size_t esize) {
+  return aligned16(p) && (size_t)ld * esize % 16 == 0;
+}
+
+}  // namespace scmp

@@ -1,0 +1,99 @@
+"""Argument checks of the layers' C entry points, which answer without a GPU."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import scmp_kernels_b200 as S
+from scmp_kernels_b200 import _layers, _lib
+
+P = 1 << 20  # a pointer that no refused call reads
+
+
+def refused(status, word):
+    assert status == _lib.SCMP_ERR_INVALID_ARG
+    assert word in _lib.lib().scmp_last_error().decode()
+
+
+def test_act8_arguments():
+    lib = _lib.lib()
+    refused(lib.scmp_act8_pack(P, 9, 1, 8, 8, P, P, None), "dtype")
+    refused(lib.scmp_act8_pack(P, 0, 1, 8, 7, P, P, None), "shape")
+    refused(lib.scmp_act8_pack(P, 0, -1, 8, 8, P, P, None), "shape")
+    refused(lib.scmp_act8_pack(None, 0, 1, 8, 8, P, P, None), "null")
+    assert lib.scmp_act8_pack(None, 0, 0, 8, 8, None, None, None) == _lib.SCMP_OK
+    refused(lib.scmp_act8_unpack(P, P, 1, 0, P, 0, None), "shape")
+    refused(lib.scmp_act8_unpack(P, None, 1, 8, P, 0, None), "null")
+
+
+def test_layer_norm_arguments():
+    lib = _lib.lib()
+    n = ctypes.c_size_t()
+    fwd = lib.scmp_layer_norm_forward
+    refused(fwd(P, 3, 1, 8, 8, None, None, 3, 1e-5, P, None, None, None, None, None), "dtype")
+    refused(fwd(P, _lib.BF16, 1, 8, 8, P, None, _lib.F16, 1e-5, P, None, None, None, None, None), "weight")
+    refused(fwd(P, 0, 1, 0, 8, None, None, 0, 1e-5, P, None, None, None, None, None), "shape")
+    refused(fwd(P, 0, 1 << 31, 8, 8, None, None, 0, 1e-5, P, None, None, None, None, None), "shape")
+    refused(fwd(P, 0, 1, 8, 4, None, None, 0, 1e-5, P, None, None, None, None, None), "ldx")
+    refused(fwd(P, 0, 1, 8, 8, None, None, 0, float("nan"), P, None, None, None, None, None), "eps")
+    refused(fwd(P, 0, 1, 8, 8, None, None, 0, 1e-5, P, None, None, P, None, None), "null")
+    bwd = lib.scmp_layer_norm_backward
+    refused(bwd(P, 8, None, 0, None, None, 0, 1, 8, P, P, None, 0, P, None, None, None, 0, None), "codes")
+    refused(bwd(P, 8, P, 8, P, P, 0, 1, 8, P, P, None, 0, P, None, None, None, 0, None), "codes")
+    refused(bwd(P, 4, P, 8, None, None, 0, 1, 8, P, P, None, 0, P, None, None, None, 0, None), "pitch")
+    refused(lib.scmp_layer_norm_backward_workspace_size(4, 0, ctypes.byref(n)), "arguments")
+    assert lib.scmp_layer_norm_backward_workspace_size(0, 8, ctypes.byref(n)) == _lib.SCMP_OK
+
+
+def test_linear_arguments():
+    lib = _lib.lib()
+    n = ctypes.c_size_t()
+    fwd = lib.scmp_linear_forward
+
+    def call(dtype=0, rows=1, d=8, m=8, act=0, bias=None, bias_dtype=0, ldx=8, ldr=0, res=None, y=P, codes=None):
+        return fwd(P, ldx, P, 8, bias, bias_dtype, res, ldr, dtype, rows, d, m, act, y, None, codes, None, None, 0, None)
+    refused(call(dtype=5), "dtype")
+    refused(call(act=5), "activation")
+    refused(call(d=0), "shape")
+    refused(call(rows=-1), "shape")
+    refused(call(bias=P, bias_dtype=2), "bias")
+    refused(call(ldx=4), "pitch")
+    refused(call(res=P, ldr=4), "pitch")
+    refused(call(y=None), "null")
+    refused(call(codes=P), "null")
+    assert call(rows=0) == _lib.SCMP_OK
+    refused(lib.scmp_linear_forward_workspace_size(0, 1, 8, 0, ctypes.byref(n)), "shape")
+    bwd = lib.scmp_linear_backward
+
+    def back(lddy=8, x=P, codes=None, act=0, pre=None, ldpre=0, w=P, bias_dtype=0):
+        return bwd(P, lddy, x, 8, codes, codes, w, 8, pre, ldpre, None, None, 0, 1, 8, 8, act, P, P, P, bias_dtype, None, 0,
+                   None)
+    refused(back(lddy=4), "pitches")
+    refused(back(x=None), "codes")
+    refused(back(codes=P), "codes")
+    refused(back(w=None), "weight")
+    refused(back(act=1), "pre")
+    refused(back(act=1, pre=P, ldpre=4), "pre")
+    refused(back(bias_dtype=1), "bias")
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(2, 8)
+    kind = ValueError if torch.cuda.is_available() else RuntimeError
+    for f in (lambda: S.pack_act8(x), lambda: S.layer_norm(x), lambda: S.linear(x, x)):
+        with pytest.raises(kind, match="CUDA"):
+            f()
+
+
+def test_rows_of_keeps_what_strides_allow():
+    t = torch.arange(240.).reshape(4, 60)
+    for v, rows, pitch, shares in [(t, 4, 60, True), (t[:, 3:20], 4, 60, True), (t[::2], 2, 120, True),
+                                   (t.t(), 60, 4, False), (t.view(2, 2, 60)[..., 1:9], 4, 60, True),
+                                   (t.view(2, 2, 60)[:, :1], 2, 60, False), (t[:, ::2], 4, 30, False),
+                                   (t[0], 1, 60, True), (t[:1].expand(4, 60), 4, 60, False)]:
+        u, r, p = _layers.rows_of(v)
+        assert (r, p) == (rows, pitch) and (u.data_ptr() == v.data_ptr()) == shares
+        flat = torch.as_strided(u, (r, v.shape[-1]), (p, 1), u.storage_offset())
+        assert torch.equal(flat, v.reshape(r, v.shape[-1]))
