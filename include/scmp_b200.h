@@ -344,8 +344,12 @@ int scmp_layer_norm_backward(const void* dy, long long lddy, const void* x, long
  * x (rows, d), weight (m, d) as sc_matmul's operands a and b. bias (m,) is
  * bias_dtype: float32 or x's type; bias and residual may be NULL. pre (rows, m)
  * and its 8-bit checkpoint pre_codes, pre_exps are written where given.
+ * Workspace sizes depend on which operands start and step by multiples of 16
+ * bytes, so that the tensor cores' loads can read them in place; `unaligned`
+ * names those that do not: 1 x, 2 weight, 4 dy (backward), added up.
  */
-int scmp_linear_forward_workspace_size(int dtype, long long rows, int d, int m, size_t* bytes);
+int scmp_linear_forward_workspace_size(int dtype, long long rows, int d, int m, int unaligned,
+                                       size_t* bytes);
 int scmp_linear_forward(const void* x, long long ldx, const void* weight, long long ldw,
                         const void* bias, int bias_dtype, const void* residual, long long ldr,
                         int dtype, long long rows, int d, int m, int activation, void* y, void* pre,
@@ -355,10 +359,11 @@ int scmp_linear_forward(const void* x, long long ldx, const void* weight, long l
  * Its gradients: dpre = dy * act'(pre), dx = dpre weight, dweight = dpre^T x,
  * dbias = column sums of dpre (the residual's gradient is dy). Each of dx,
  * dweight and dbias may be NULL. x (for dweight) and pre (for an activation)
- * are given as tensors or as 8-bit checkpoints.
+ * are given as tensors or as 8-bit checkpoints. Workspace: parts is the sum of 1
+ * (dx), 2 (dweight) and 4 (dbias) that will be asked for.
  */
 int scmp_linear_backward_workspace_size(int dtype, long long rows, int d, int m, int activation,
-                                        int x_packed, int with_bias, size_t* bytes);
+                                        int x_packed, int parts, int unaligned, size_t* bytes);
 int scmp_linear_backward(const void* dy, long long lddy, const void* x, long long ldx,
                          const int8_t* x_codes, const uint8_t* x_exps, const void* weight,
                          long long ldw, const void* pre, long long ldpre, const int8_t* pre_codes,

@@ -100,5 +100,11 @@ def workspace(device: torch.device, name: str, *sizes: int):
     return ws.data_ptr(), n, ws
 
 
+def unaligned(flag: int, t, pitch: int) -> int:
+    """``flag`` when the library has to copy ``t``'s rows before it can multiply
+    them (they do not start and step by 16 bytes), else 0."""
+    return flag if t is not None and (t.data_ptr() | pitch * t.element_size()) & 15 else 0
+
+
 def ptr(t):
     return None if t is None else t.data_ptr()

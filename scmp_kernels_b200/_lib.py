@@ -107,11 +107,11 @@ SIGNATURES = {
     "scmp_layer_norm_backward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int,
                                          c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_size_t, c_void_p]),
-    "scmp_linear_forward_workspace_size": (c_int, [c_int, c_longlong, c_int, c_int, ctypes.POINTER(c_size_t)]),
+    "scmp_linear_forward_workspace_size": (c_int, [c_int, c_longlong, c_int, c_int, c_int, ctypes.POINTER(c_size_t)]),
     "scmp_linear_forward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_longlong,
                                     c_int, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_size_t, c_void_p]),
-    "scmp_linear_backward_workspace_size": (c_int, [c_int, c_longlong, c_int, c_int, c_int, c_int, c_int,
+    "scmp_linear_backward_workspace_size": (c_int, [c_int, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int,
                                                     ctypes.POINTER(c_size_t)]),
     "scmp_linear_backward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p,
                                      c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int,

@@ -57,7 +57,8 @@ __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x,
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) act8_unpack_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
-                                                          long long rows, int cols, T* __restrict__ out) {
+                                                          long long rows, int cols, long long ldo,
+                                                          T* __restrict__ out) {
   const int nb = act8_blocks(cols);
   const long long total = rows * nb * 4;
   const long long stride = (long long)gridDim.x * blockDim.x;
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const int8_t* __restri
     if (c0 >= cols) continue;
     const float s = act8_scale(__ldg(exps + blk));
     const int8_t* src = codes + row * cols + c0;
-    T* dst = out + row * cols + c0;
+    T* dst = out + row * ldo + c0;
     if (VEC) {
       const uint2 q = __ldg(reinterpret_cast<const uint2*>(src));
       float v[8];
@@ -88,15 +89,15 @@ static int elementwise_grid(long long items, int per_block) {
 }
 
 cudaError_t launch_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, int cols, void* out,
-                                      int dtype, cudaStream_t st) {
-  const bool vec = cols % 8 == 0 && aligned16(codes) && aligned16(out);
+                               long long ldo, int dtype, cudaStream_t st) {
+  const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && rows_aligned16(out, ldo, dtype_size(dtype));
   const int grid = elementwise_grid(rows * act8_blocks(cols) * 4, 256);
   with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     if (vec)
-      act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, exps, rows, cols, (T*)out);
+      act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, exps, rows, cols, ldo, (T*)out);
     else
-      act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, exps, rows, cols, (T*)out);
+      act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, exps, rows, cols, ldo, (T*)out);
   });
   count_launch();
   return cudaGetLastError();
@@ -135,7 +136,7 @@ int scmp_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, i
   if (rows < 0 || cols < 1) return fail(SCMP_ERR_INVALID_ARG, "act8_unpack: bad shape (rows >= 0, cols >= 1)");
   if (rows == 0) return SCMP_OK;
   if (!codes || !exps || !out) return fail(SCMP_ERR_INVALID_ARG, "act8_unpack: null pointer");
-  SCMP_CUDA(launch_act8_unpack(codes, exps, rows, cols, out, dtype, (cudaStream_t)stream), "act8_unpack");
+  SCMP_CUDA(launch_act8_unpack(codes, exps, rows, cols, out, cols, dtype, (cudaStream_t)stream), "act8_unpack");
   return SCMP_OK;
 }
 

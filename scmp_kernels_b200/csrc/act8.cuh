@@ -47,9 +47,9 @@ __device__ __forceinline__ int act8_code(float x, float inverse, bool nan_block)
   return nan_block ? 0 : c;
 }
 
-// The values of a checkpoint as a contiguous tensor of type dtype (act8.cu).
-cudaError_t launch_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, int cols, void* out, int dtype,
-                               cudaStream_t st);
+// The values of a checkpoint as rows of type dtype at a pitch of ldo (act8.cu).
+cudaError_t launch_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, int cols, void* out,
+                               long long ldo, int dtype, cudaStream_t st);
 
 // out_k[c] = sum over p < parts of part[p][k][c], k < sets <= 2, in a fixed
 // order, as dtype; a null out is skipped (layer_norm.cu).

@@ -16,9 +16,40 @@ struct DpreArgs {
   const uint8_t* exps;
   long long rows, ldy, ldp;
   int cols, act;
-  void* dpre;   // (rows, cols), or null (no activation: dy itself is dpre)
+  void* dpre;   // rows at a pitch of ldo 16-bit values, float32 as three planes; or null
+  long long ldo;
   float* part;  // (gridDim.y, cols), or null
 };
+template <class T>
+__device__ __forceinline__ void store_operand8(void* out, long long plane, long long at, const float (&d)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    stg8((T*)out + at, d);
+  } else {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      uint32_t lo[3], hi[3];
+      split3(d[i], lo);
+      split3(d[i + 1], hi);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) w[p][i >> 1] = lo[p] | (hi[p] << 16);
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      *reinterpret_cast<uint4*>((uint16_t*)out + p * plane + at) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_operand1(void* out, long long plane, long long at, float v) {
+  if constexpr (sizeof(T) == 2) {
+    ((T*)out)[at] = Elem<T>::from_f(v);
+  } else {
+    uint32_t p[3];
+    split3(v, p);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) ((uint16_t*)out)[i * plane + at] = (uint16_t)p[i];
+  }
+}
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
   __shared__ float s[8][256];
@@ -46,7 +77,7 @@ __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) d[j] *= act_grad(a.act, p[j]);
         }
-        if (a.dpre) stg8((T*)a.dpre + row * a.cols + cv, d);
+        if (a.dpre) store_operand8<T>(a.dpre, a.rows * a.ldo, row * a.ldo + cv, d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += d[j];
       }
@@ -61,7 +92,7 @@ __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
                                   : ldg1((const T*)a.pre + row * a.ldp + c);
           v *= act_grad(a.act, q);
         }
-        if (a.dpre) ((T*)a.dpre)[row * a.cols + c] = Elem<T>::from_f(v);
+        if (a.dpre) store_operand1<T>(a.dpre, a.rows * a.ldo, row * a.ldo + c, v);
         sum[j] += v;
       }
     }
@@ -108,20 +139,69 @@ struct Carve {
     return p;
   }
 };
+// Bytes of a (rows, cols) operand staged for the product.
+static size_t staged_bytes(int dtype, long long rows, int cols) {
+  return (size_t)rows * pitch_of(cols) * 2 * (dtype == SCMP_F32 ? 3 : 1);
+}
+// Operands that are staged: float32 ones, and those TMA cannot read in place.
+constexpr int kUnalignedX = 1, kUnalignedWeight = 2, kUnalignedDy = 4;
+static int unaligned(const void* p, long long ld, int dtype, int flag) {
+  return rows_aligned16(p, ld, dtype_size(dtype)) ? 0 : flag;
+}
+
+struct ForwardPlan {
+  char* x;
+  char* w;
+  char* partial;
+};
+static ForwardPlan plan_forward(Carve& c, int dtype, long long rows, int d, int m, int unal) {
+  ForwardPlan p{};
+  const bool f32 = dtype == SCMP_F32;
+  if (f32 || (unal & kUnalignedX)) p.x = c.take<char>(staged_bytes(dtype, rows, d));
+  if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(dtype, m, d));
+  p.partial = c.take<char>(partial_bytes(rows, m, (d + KB - 1LL) / KB * (f32 ? 6 : 1)));
+  return p;
+}
 struct BackwardPlan {
-  char* dpre;   // dpre in the tensors' type (with an activation)
-  char* x;      // x unpacked from its checkpoint
+  char* dpre;   // dpre, or dy staged
+  char* x;      // x staged, or unpacked from its checkpoint (exact in 16 bits)
+  char* w;      // weight staged
+  char* partial;
   float* part;  // column sums of dpre per block row
   int row_blocks;
 };
-static BackwardPlan plan_backward(Carve& c, int dtype, long long rows, int d, int m, int act, bool x8, bool with_bias) {
-  const size_t es = dtype_size(dtype);
+// parts: bit 0 dx, bit 1 dweight, bit 2 dbias
+static BackwardPlan plan_backward(Carve& c, int dtype, long long rows, int d, int m, int act, bool x8, int parts, int unal) {
   BackwardPlan p{};
+  const bool f32 = dtype == SCMP_F32;
   p.row_blocks = dpre_row_blocks(rows, m);
-  if (act != SCMP_ACT_NONE) p.dpre = c.take<char>(rows * m * es);
-  if (x8) p.x = c.take<char>(rows * d * es);
-  if (with_bias) p.part = c.take<float>((size_t)p.row_blocks * m);
+  if ((parts & 3) && (act != SCMP_ACT_NONE || f32 || (unal & kUnalignedDy))) p.dpre = c.take<char>(staged_bytes(dtype, rows, m));
+  size_t partial = 0;
+  if (parts & 2) {
+    if (x8)
+      p.x = c.take<char>(staged_bytes(SCMP_BF16, rows, d));
+    else if (f32 || (unal & kUnalignedX))
+      p.x = c.take<char>(staged_bytes(dtype, rows, d));
+    partial = partial_bytes(m, d, (rows + KB - 1) / KB * (f32 ? (x8 ? 3 : 6) : 1));
+  }
+  if (parts & 1) {
+    if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(dtype, m, d));
+    const size_t q = partial_bytes(rows, d, (m + KB - 1LL) / KB * (f32 ? 6 : 1));
+    if (q > partial) partial = q;
+  }
+  p.partial = c.take<char>(partial);
+  if (parts & 4) p.part = c.take<float>((size_t)p.row_blocks * m);
   return p;
+}
+// The operand of a (rows, cols) tensor, staged into `room` when it has to be.
+static cudaError_t operand(const void* p, long long ld, long long rows, int cols, int dtype, char* room, bool mn, Operand& o,
+                           cudaStream_t st) {
+  o = {p, cols, rows, ld, 1, mn};
+  if (!room) return cudaSuccess;
+  o.p = room;
+  o.ld = pitch_of(cols);
+  o.planes = dtype == SCMP_F32 ? 3 : 1;
+  return launch_restage(p, rows, cols, ld, dtype, room, st);
 }
 
 static int check_shape(const char* who, int dtype, long long rows, int d, int m, int act) {
@@ -140,10 +220,12 @@ using namespace scmp;
 
 extern "C" {
 
-int scmp_linear_forward_workspace_size(int dtype, long long rows, int d, int m, size_t* bytes) {
+int scmp_linear_forward_workspace_size(int dtype, long long rows, int d, int m, int unaligned, size_t* bytes) {
   if (int e = lin::check_shape("linear_forward_workspace_size", dtype, rows, d, m, 0)) return e;
   if (!bytes) return fail(SCMP_ERR_INVALID_ARG, "linear_forward_workspace_size: null pointer");
-  *bytes = 0;
+  lin::Carve c{nullptr};
+  lin::plan_forward(c, dtype, rows, d, m, unaligned);
+  *bytes = c.off;
   return SCMP_OK;
 }
 
@@ -157,18 +239,25 @@ int scmp_linear_forward(const void* x, long long ldx, const void* weight, long l
   if (ldx < d || ldw < d || (residual && ldr < m)) return fail(SCMP_ERR_INVALID_ARG, "linear_forward: row pitch too small");
   if (rows == 0) return SCMP_OK;
   if (!x || !weight || !y || !pre_codes != !pre_exps) return fail(SCMP_ERR_INVALID_ARG, "linear_forward: null pointer");
-  lin::Product p{x, weight, ldx, 1, ldw, 1, (int)rows, m, d};
-  lin::Epilogue e{bias, bias_dtype == SCMP_F32, residual, ldr, activation, y, m, pre, pre_codes, pre_exps};
-  SCMP_CUDA(lin::launch_gemm(p, e, dtype, (cudaStream_t)stream), "linear_forward");
+  const cudaStream_t st = (cudaStream_t)stream;
+  lin::Carve c{(char*)workspace};
+  const int unal = lin::unaligned(x, ldx, dtype, lin::kUnalignedX) | lin::unaligned(weight, ldw, dtype, lin::kUnalignedWeight);
+  const lin::ForwardPlan w = lin::plan_forward(c, dtype, rows, d, m, unal);
+  if (c.off && (!workspace || workspace_bytes < c.off)) return fail(SCMP_ERR_WORKSPACE, "linear_forward: workspace missing or too small");
+  lin::Operand a, b;
+  SCMP_CUDA(lin::operand(x, ldx, rows, d, dtype, w.x, false, a, st), "linear_forward: x");
+  SCMP_CUDA(lin::operand(weight, ldw, m, d, dtype, w.w, false, b, st), "linear_forward: weight");
+  const lin::Epilogue e{bias, bias_dtype == SCMP_F32, residual, ldr, activation, y, m, pre, pre_codes, pre_exps};
+  SCMP_CUDA(lin::launch_tc(a, b, rows, m, d, e, dtype, (float*)w.partial, st), "linear_forward");
   return SCMP_OK;
 }
 
-int scmp_linear_backward_workspace_size(int dtype, long long rows, int d, int m, int activation, int x_packed,
-                                        int with_bias, size_t* bytes) {
+int scmp_linear_backward_workspace_size(int dtype, long long rows, int d, int m, int activation, int x_packed, int parts,
+                                        int unaligned, size_t* bytes) {
   if (int e = lin::check_shape("linear_backward_workspace_size", dtype, rows, d, m, activation)) return e;
   if (!bytes) return fail(SCMP_ERR_INVALID_ARG, "linear_backward_workspace_size: null pointer");
   lin::Carve c{nullptr};
-  lin::plan_backward(c, dtype, rows, d, m, activation, x_packed != 0, with_bias != 0);
+  lin::plan_backward(c, dtype, rows, d, m, activation, x_packed != 0, parts, unaligned);
   *bytes = c.off;
   return SCMP_OK;
 }
@@ -180,51 +269,60 @@ int scmp_linear_backward(const void* dy, long long lddy, const void* x, long lon
                          size_t workspace_bytes, void* stream) {
   if (int e = lin::check_shape("linear_backward", dtype, rows, d, m, activation)) return e;
   const cudaStream_t st = (cudaStream_t)stream;
-  const size_t es = dtype_size(dtype);
   if (dbias && bias_dtype != dtype && bias_dtype != SCMP_F32)
     return fail(SCMP_ERR_INVALID_ARG, "linear_backward: the bias is float32 or dy's type");
   if (rows == 0) {
-    if (dweight) SCMP_CUDA(cudaMemsetAsync(dweight, 0, (size_t)m * d * es, st), "linear_backward");
+    if (dweight) SCMP_CUDA(cudaMemsetAsync(dweight, 0, (size_t)m * d * dtype_size(dtype), st), "linear_backward");
     if (dbias) SCMP_CUDA(cudaMemsetAsync(dbias, 0, (size_t)m * dtype_size(bias_dtype), st), "linear_backward");
     return SCMP_OK;
   }
-  if (!dy || lddy < m || (dx && (!weight || ldw < d)) || (dweight && !x == !x_codes) || !x_codes != !x_exps || (x && ldx < d))
+  if (!dy || lddy < m || (dx && (!weight || ldw < d)) || (dweight && !x == !x_codes) || !x_codes != !x_exps ||
+      (dweight && x && ldx < d))
     return fail(SCMP_ERR_INVALID_ARG, "linear_backward: give dy, weight (for dx) and x or its codes and exps (for dweight), at pitches that hold a row");
   const bool act = activation != SCMP_ACT_NONE;
   if (act && (!pre == !pre_codes || !pre_codes != !pre_exps || (pre && ldpre < m)))
     return fail(SCMP_ERR_INVALID_ARG, "linear_backward: an activation's gradient needs pre, or its codes and exps");
+  const int parts = (dx ? 1 : 0) | (dweight ? 2 : 0) | (dbias ? 4 : 0);
+  if (!parts) return SCMP_OK;
+  const bool x8 = dweight && x_codes;
+  int unal = lin::unaligned(dy, lddy, dtype, lin::kUnalignedDy);
+  if (dweight && !x8) unal |= lin::unaligned(x, ldx, dtype, lin::kUnalignedX);
+  if (dx) unal |= lin::unaligned(weight, ldw, dtype, lin::kUnalignedWeight);
   lin::Carve c{(char*)workspace};
-  const lin::BackwardPlan w = lin::plan_backward(c, dtype, rows, d, m, activation, x_codes != nullptr, dbias != nullptr);
+  const lin::BackwardPlan w = lin::plan_backward(c, dtype, rows, d, m, activation, x8, parts, unal);
   if (c.off && (!workspace || workspace_bytes < c.off)) return fail(SCMP_ERR_WORKSPACE, "linear_backward: workspace missing or too small");
-  const void* g = dy;
-  long long ldg = lddy;
+  lin::Operand g{dy, m, rows, lddy, 1, false};
   if (act || dbias) {
-    lin::DpreArgs a{dy, pre, pre_codes, pre_exps, rows, lddy, ldpre, m, activation, act ? w.dpre : nullptr, w.part};
+    lin::DpreArgs a{dy, pre, pre_codes, pre_exps, rows, lddy, ldpre, m, activation, w.dpre, lin::pitch_of(m), w.part};
     SCMP_CUDA(lin::launch_dpre(a, dtype, w.row_blocks, st), "linear_backward: activation");
     if (dbias)
       SCMP_CUDA(launch_column_sum(w.part, w.row_blocks, 1, m, bias_dtype, dbias, nullptr, st), "linear_backward: bias");
-    if (act) { g = w.dpre; ldg = m; }
+    if (w.dpre) g = {w.dpre, m, rows, lin::pitch_of(m), dtype == SCMP_F32 ? 3 : 1, false};
+  } else {
+    SCMP_CUDA(lin::operand(dy, lddy, rows, m, dtype, w.dpre, false, g, st), "linear_backward: dy");
   }
   if (dx) {
-    lin::Product p{g, weight, ldg, 1, 1, ldw, (int)rows, d, m};
+    lin::Operand b;
+    SCMP_CUDA(lin::operand(weight, ldw, m, d, dtype, w.w, true, b, st), "linear_backward: weight");
     lin::Epilogue e{};
     e.out = dx;
     e.ldo = d;
-    SCMP_CUDA(lin::launch_gemm(p, e, dtype, st), "linear_backward: dx");
+    SCMP_CUDA(lin::launch_tc(g, b, rows, d, m, e, dtype, (float*)w.partial, st), "linear_backward: dx");
   }
   if (dweight) {
-    const void* xs = x;
-    long long lx = ldx;
-    if (x_codes) {
-      SCMP_CUDA(launch_act8_unpack(x_codes, x_exps, rows, d, w.x, dtype, st), "linear_backward: unpack");
-      xs = w.x;
-      lx = d;
+    lin::Operand b;
+    if (x8) {
+      const int t = dtype == SCMP_F32 ? SCMP_BF16 : dtype;
+      SCMP_CUDA(launch_act8_unpack(x_codes, x_exps, rows, d, w.x, lin::pitch_of(d), t, st), "linear_backward: unpack");
+      b = {w.x, d, rows, lin::pitch_of(d), 1, true};
+    } else {
+      SCMP_CUDA(lin::operand(x, ldx, rows, d, dtype, w.x, true, b, st), "linear_backward: x");
     }
-    lin::Product p{g, xs, 1, ldg, 1, lx, m, d, (int)rows};
+    g.mn = true;
     lin::Epilogue e{};
     e.out = dweight;
     e.ldo = d;
-    SCMP_CUDA(lin::launch_gemm(p, e, dtype, st), "linear_backward: dweight");
+    SCMP_CUDA(lin::launch_tc(g, b, m, d, rows, e, dtype, (float*)w.partial, st), "linear_backward: dweight");
   }
   return SCMP_OK;
 }

@@ -59,13 +59,20 @@ struct Epilogue {
   uint8_t* exps;
 };
 
-// C(i, j) = sum over k of A(i, k) * B(j, k): A at a[i * ai + k * ak], B likewise.
-struct Product {
-  const void* a;
-  const void* b;
-  long long ai, ak, bj, bk;
-  int m, n, k;
-};
+// A float32 value as three bfloat16 (leading 8 bits, the next 8, the last 8)
+// whose sum it is. Truncated, so that no part overflows; an infinity or a NaN is
+// the first part alone.
+__device__ __forceinline__ void split3(float v, uint32_t (&part)[3]) {
+  uint32_t u = __float_as_uint(v);
+  const bool finite = (u & 0x7F800000u) != 0x7F800000u;
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) u |= 0x00400000u;  // a NaN keeps a set mantissa bit
+  part[0] = u >> 16;
+  v = finite ? v - __uint_as_float(u & 0xFFFF0000u) : 0.f;
+  u = __float_as_uint(v);
+  part[1] = u >> 16;
+  v -= __uint_as_float(u & 0xFFFF0000u);
+  part[2] = __float_as_uint(v) >> 16;
+}
 
 }  // namespace lin
 }  // namespace scmp

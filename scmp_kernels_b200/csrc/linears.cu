@@ -1,5 +1,5 @@
 // Translation unit of the exact linear layer.
-#include "linear_gemm.cu"
+#include "linear_tc.cu"
 #include "linear.cu"
 
 namespace scmp {

@@ -74,7 +74,8 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
         y = torch.empty(shape, dtype=x.dtype, device=dev)
         pre = torch.empty(shape, dtype=x.dtype, device=dev) if save == "exact" else \
             _empty(shape, x.dtype, dev) if save == "8bit" else None
-        ws, nbytes, keep = L.workspace(dev, "scmp_linear_forward_workspace_size", dt, rows, d, m)
+        ws, nbytes, keep = L.workspace(dev, "scmp_linear_forward_workspace_size", dt, rows, d, m,
+                                       L.unaligned(1, x2, ldx) | L.unaligned(2, w2, ldw))
         L.call("scmp_linear_forward", x2.data_ptr(), ldx, w2.data_ptr(), ldw, L.ptr(bias),
                dt if bias is None else L.DTYPES[bias.dtype], L.ptr(r2), ldr, dt, rows, d, m, act, y.data_ptr(),
                pre.data_ptr() if save == "exact" else None, pre.codes.data_ptr() if save == "8bit" else None,
@@ -140,14 +141,13 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Act8, None], weight
         dx = torch.empty((*lead, d), dtype=dy.dtype, device=dev) if need_dx else None
         dw = torch.empty((m, d), dtype=dy.dtype, device=dev) if need_dweight else None
         db = torch.empty(m, dtype=bias_dtype, device=dev) if with_bias else None
-        if d is not None:
-            ws, nbytes, keep = L.workspace(dev, "scmp_linear_backward_workspace_size", dt, rows, d, m, act,
-                                           int(x8 is not None), int(with_bias))
-        elif with_bias:
-            d = 1
-            ws, nbytes, keep = L.workspace(dev, "scmp_linear_backward_workspace_size", dt, rows, d, m, act, 0, 1)
-        else:
+        parts = int(need_dx) | 2 * int(need_dweight) | 4 * int(with_bias)
+        if not parts:
             return None, None, None
+        d = 1 if d is None else d
+        ws, nbytes, keep = L.workspace(dev, "scmp_linear_backward_workspace_size", dt, rows, d, m, act,
+                                       int(x8 is not None), parts,
+                                       L.unaligned(4, dy2, ldy) | L.unaligned(1, x2, ldx) | L.unaligned(2, w2, ldw))
         L.call("scmp_linear_backward", dy2.data_ptr(), ldy, L.ptr(x2), ldx, x8.codes.data_ptr() if x8 is not None else None,
                x8.exponents.data_ptr() if x8 is not None else None, L.ptr(w2), ldw, L.ptr(p2), ldp,
                p8.codes.data_ptr() if p8 is not None else None, p8.exponents.data_ptr() if p8 is not None else None, dt,

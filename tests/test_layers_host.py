@@ -64,7 +64,7 @@ def test_linear_arguments():
     refused(call(y=None), "null")
     refused(call(codes=P), "null")
     assert call(rows=0) == _lib.SCMP_OK
-    refused(lib.scmp_linear_forward_workspace_size(0, 1, 8, 0, ctypes.byref(n)), "shape")
+    refused(lib.scmp_linear_forward_workspace_size(0, 1, 8, 0, 0, ctypes.byref(n)), "shape")
     bwd = lib.scmp_linear_backward
 
     def back(lddy=8, x=P, codes=None, act=0, pre=None, ldpre=0, w=P, bias_dtype=0):
