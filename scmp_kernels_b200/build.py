@@ -23,7 +23,7 @@ UNITS = {
     "scmp_b200": ["scmp_b200.cu", "tables.cu", "quant.cu", "gemm_simt.cu", "gemm_tc.cu", "api.cu", "levels.cu",
                   "quant_ref.cu", "noalloc.cu"],
     "norms": ["norms.cu", "act8.cu", "layer_norm.cu"],
-    "linears": ["linears.cu", "linear_tc.cu", "linear.cu"],
+    "linears": ["linears.cu", "linear_rows.cu", "linear_tc.cu", "linear.cu"],
 }
 # Headers that only some units include.
 UNIT_HEADERS = {"internal.cuh": ("scmp_b200",), "quant.cuh": ("scmp_b200",), "vecio.cuh": ("norms", "linears"),

@@ -330,25 +330,27 @@ __global__ void __launch_bounds__(block_threads<TPR>()) backward_kernel(Args a) 
   }
 }
 
-// out_k[c] = sum over p of part[p][k][c], in order of p within eight strands.
+// out_k[c] = sum over p of part[p][k][c]: 32 strands of p per column, each in
+// order, then the strands in order.
 template <class W>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ part, int parts, int sets, int cols,
-                                                         W* __restrict__ out0, W* __restrict__ out1) {
-  __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, int parts, int sets, int cols,
+                                                          W* __restrict__ out0, W* __restrict__ out1) {
+  __shared__ float s[32][33];
   const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lx, k = blockIdx.y;
   W* out = k ? out1 : out0;
   if (!out) return;
   float v = 0.f;
-  if (c < cols)
-    for (int p = ly; p < parts; p += 8) v += part[((size_t)p * sets + k) * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (int p = ly; p < parts; p += 32) v += __ldg(part + ((size_t)p * sets + k) * cols + c);
+  }
   s[ly][lx] = v;
   __syncthreads();
-  if (ly == 0 && c < cols) {
+  v = s[lx][ly];  // a warp per column
 #pragma unroll
-    for (int y = 1; y < 8; ++y) v += s[y][lx];
-    out[c] = Elem<W>::from_f(v);
-  }
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_down_sync(0xffffffffu, v, o);
+  if (lx == 0 && blockIdx.x * 32 + ly < cols) out[blockIdx.x * 32 + ly] = Elem<W>::from_f(v);
 }
 
 // Rows longer than kMaxFused: one block per row, the row read once per pass.
@@ -537,7 +539,7 @@ cudaError_t launch_column_sum(const float* part, int parts, int sets, int cols, 
                                      cudaStream_t st) {
   with_dtype(dtype, [&](auto* tag) {
     using W = std::remove_pointer_t<decltype(tag)>;
-    ln::column_sum_kernel<W><<<dim3(cdiv(cols, 32), sets), 256, 0, st>>>(part, parts, sets, cols, (W*)out0, (W*)out1);
+    ln::column_sum_kernel<W><<<dim3(cdiv(cols, 32), sets), 1024, 0, st>>>(part, parts, sets, cols, (W*)out0, (W*)out1);
   });
   count_launch();
   return cudaGetLastError();

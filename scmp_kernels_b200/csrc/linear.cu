@@ -50,6 +50,29 @@ __device__ __forceinline__ void store_operand1(void* out, long long plane, long 
     for (int i = 0; i < 3; ++i) ((uint16_t*)out)[i * plane + at] = (uint16_t)p[i];
   }
 }
+// Raw values of a thread's eight columns of a row.
+template <class T>
+struct DpreRaw {
+  Raw8<T> dy, pre;
+  uint2 codes;
+  uint8_t ex;
+};
+template <class T>
+__device__ __forceinline__ void dpre_load(const DpreArgs& a, long long row, int c, DpreRaw<T>& r) {
+  r.dy = ldg8((const T*)a.dy + row * a.ldy + c);
+  if (a.act == SCMP_ACT_NONE) return;
+  if (a.codes) {
+    r.codes = __ldg(reinterpret_cast<const uint2*>(a.codes + row * a.cols + c));
+    r.ex = __ldg(a.exps + row * act8_blocks(a.cols) + (c >> 5));
+  } else {
+    r.pre = ldg8((const T*)a.pre + row * a.ldp + c);
+  }
+}
+template <int ACT>
+__device__ __forceinline__ void times_grad(float (&d)[8], const float (&p)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) d[j] *= act_grad(ACT, p[j]);
+}
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
   __shared__ float s[8][256];
@@ -58,42 +81,58 @@ __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
   float sum[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) sum[j] = 0.f;
-  for (long long row = (long long)blockIdx.y * 8 + group; row < a.rows; row += (long long)gridDim.y * 8) {
-    const T* dy = (const T*)a.dy + row * a.ldy;
-    float d[8], p[8];
-    const int cv = c0 + lane * 8;
-    if (VEC) {
-      if (cv < a.cols) {
-        unpack8(ldg8(dy + cv), d);
+  const long long step = (long long)gridDim.y * 8;
+  if (VEC) {
+    const int c = c0 + lane * 8;
+    long long row = (long long)blockIdx.y * 8 + group;
+    if (c < a.cols && row < a.rows) {
+      DpreRaw<T> next;
+      dpre_load<T>(a, row, c, next);
+      for (; row < a.rows; row += step) {  // the next row's loads run under this row's arithmetic
+        const DpreRaw<T> cur = next;
+        if (row + step < a.rows) dpre_load<T>(a, row + step, c, next);
+        float d[8], p[8];
+        unpack8(cur.dy, d);
         if (a.act != SCMP_ACT_NONE) {
           if (a.codes) {
-            const uint2 q = __ldg(reinterpret_cast<const uint2*>(a.codes + row * a.cols + cv));
-            const float sc = act8_scale(__ldg(a.exps + row * act8_blocks(a.cols) + (cv >> 5)));
+            const float sc = act8_scale(cur.ex);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = fmul((float)(int8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3))), sc);
+            for (int j = 0; j < 8; ++j) p[j] = fmul((float)(int8_t)((j < 4 ? cur.codes.x : cur.codes.y) >> (8 * (j & 3))), sc);
           } else {
-            unpack8(ldg8((const T*)a.pre + row * a.ldp + cv), p);
+            unpack8(cur.pre, p);
           }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) d[j] *= act_grad(a.act, p[j]);
+          switch (a.act) {
+            case SCMP_ACT_RELU: times_grad<SCMP_ACT_RELU>(d, p); break;
+            case SCMP_ACT_GELU: times_grad<SCMP_ACT_GELU>(d, p); break;
+            case SCMP_ACT_GELU_TANH: times_grad<SCMP_ACT_GELU_TANH>(d, p); break;
+            default: times_grad<SCMP_ACT_SILU>(d, p);
+          }
         }
-        if (a.dpre) store_operand8<T>(a.dpre, a.rows * a.ldo, row * a.ldo + cv, d);
+        if (a.dpre) store_operand8<T>(a.dpre, a.rows * a.ldo, row * a.ldo + c, d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += d[j];
       }
-    } else {
+    }
+  } else {
+    for (long long row = (long long)blockIdx.y * 8 + group; row < a.rows; row += step) {
+      const T* dy = (const T*)a.dy + row * a.ldy;
+      float v[8], q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = c0 + j * 32 + lane;
+        v[j] = c < a.cols ? ldg1(dy + c) : 0.f;
+        q[j] = 0.f;
+        if (a.act != SCMP_ACT_NONE && c < a.cols)
+          q[j] = a.codes ? fmul((float)__ldg(a.codes + row * a.cols + c), act8_scale(__ldg(a.exps + row * act8_blocks(a.cols) + (c >> 5))))
+                         : ldg1((const T*)a.pre + row * a.ldp + c);
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int c = c0 + j * 32 + lane;
         if (c >= a.cols) continue;
-        float v = ldg1(dy + c);
-        if (a.act != SCMP_ACT_NONE) {
-          const float q = a.codes ? fmul((float)a.codes[row * a.cols + c], act8_scale(a.exps[row * act8_blocks(a.cols) + (c >> 5)]))
-                                  : ldg1((const T*)a.pre + row * a.ldp + c);
-          v *= act_grad(a.act, q);
-        }
-        if (a.dpre) store_operand1<T>(a.dpre, a.rows * a.ldo, row * a.ldo + c, v);
-        sum[j] += v;
+        if (a.act != SCMP_ACT_NONE) v[j] *= act_grad(a.act, q[j]);
+        if (a.dpre) store_operand1<T>(a.dpre, a.rows * a.ldo, row * a.ldo + c, v[j]);
+        sum[j] += v[j];
       }
     }
   }
@@ -150,12 +189,15 @@ static int unaligned(const void* p, long long ld, int dtype, int flag) {
 }
 
 struct ForwardPlan {
+  bool rows;  // the kernel for a few rows, which needs no workspace
   char* x;
   char* w;
   char* partial;
 };
 static ForwardPlan plan_forward(Carve& c, int dtype, long long rows, int d, int m, int unal) {
   ForwardPlan p{};
+  p.rows = few_rows(dtype, rows);
+  if (p.rows) return p;
   const bool f32 = dtype == SCMP_F32;
   if (f32 || (unal & kUnalignedX)) p.x = c.take<char>(staged_bytes(dtype, rows, d));
   if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(dtype, m, d));
@@ -244,10 +286,14 @@ int scmp_linear_forward(const void* x, long long ldx, const void* weight, long l
   const int unal = lin::unaligned(x, ldx, dtype, lin::kUnalignedX) | lin::unaligned(weight, ldw, dtype, lin::kUnalignedWeight);
   const lin::ForwardPlan w = lin::plan_forward(c, dtype, rows, d, m, unal);
   if (c.off && (!workspace || workspace_bytes < c.off)) return fail(SCMP_ERR_WORKSPACE, "linear_forward: workspace missing or too small");
+  const lin::Epilogue e{bias, bias_dtype == SCMP_F32, residual, ldr, activation, y, m, pre, pre_codes, pre_exps};
+  if (w.rows) {
+    SCMP_CUDA(lin::launch_rows(x, ldx, weight, ldw, (int)rows, d, m, e, dtype, st), "linear_forward");
+    return SCMP_OK;
+  }
   lin::Operand a, b;
   SCMP_CUDA(lin::operand(x, ldx, rows, d, dtype, w.x, false, a, st), "linear_forward: x");
   SCMP_CUDA(lin::operand(weight, ldw, m, d, dtype, w.w, false, b, st), "linear_forward: weight");
-  const lin::Epilogue e{bias, bias_dtype == SCMP_F32, residual, ldr, activation, y, m, pre, pre_codes, pre_exps};
   SCMP_CUDA(lin::launch_tc(a, b, rows, m, d, e, dtype, (float*)w.partial, st), "linear_forward");
   return SCMP_OK;
 }

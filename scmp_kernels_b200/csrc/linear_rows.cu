@@ -1,0 +1,260 @@
+// The linear layer for a few rows (decoded tokens): y = act(x w^T + bias) + residual.
+//
+// With R rows every weight is used R times, so the weight's way from memory
+// bounds it: D * M values once, whatever R. A block takes 16 weight rows, its
+// warps share their columns evenly, and the partial sums meet in shared memory
+// in warp order. Weights and x go from global memory straight into registers, 16
+// bytes per lane. 16-bit types use mma.sync with the weight rows as the
+// 16-row operand and the tokens as the 8 columns (tcgen05 would need the
+// operands in shared memory first and a tile of at least 64 rows, and gains
+// nothing where memory is the bound). The order of a sum's terms is free, so
+// a lane's eight consecutive values serve as the fragment's k pairs as they
+// come. float32 multiplies on the CUDA cores.
+#include "linear.cuh"
+#include "status.cuh"
+
+namespace scmp {
+namespace lin {
+
+constexpr int ROWS_WARPS = 8;
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1, const __nv_bfloat16*) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1, const __half*) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Eight 16-bit values of a row from column c; zeros past the row's end and for
+// rows that do not exist.
+template <bool VEC>
+__device__ __forceinline__ uint4 load16(const uint16_t* row, int c, int cols, bool live) {
+  uint4 q = make_uint4(0, 0, 0, 0);
+  if (VEC) {
+    if (live && c < cols) q = __ldg(reinterpret_cast<const uint4*>(row + c));
+  } else if (live) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&q);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) w[i >> 1] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(row) + c + i) << (16 * (i & 1));
+  }
+  return q;
+}
+
+struct RowsArgs {
+  const void* x;
+  const void* w;
+  long long ldx, ldw;
+  int rows, d, m;
+  Epilogue e;
+};
+
+// Row r, column j of the result, a lane per column (a warp's 32 columns are one
+// block of an 8-bit checkpoint when it is asked for).
+template <class T>
+__device__ __forceinline__ void finish_element(const RowsArgs& a, float v, int r, int j, bool live) {
+  const Epilogue& e = a.e;
+  if (e.bias && live) v += e.bias_f32 ? __ldg((const float*)e.bias + j) : ldg1((const T*)e.bias + j);
+  if (e.pre && live) ((T*)e.pre)[(long long)r * a.m + j] = Elem<T>::from_f(v);
+  if (e.codes) {
+    const uint32_t byte = act8_exponent(__reduce_max_sync(0xffffffffu, live ? __float_as_uint(v) & 0x7FFFFFFFu : 0u), act8_floor<T>());
+    if (live) e.codes[(long long)r * a.m + j] = (int8_t)act8_code(v, act8_inverse(byte), byte == kAct8Nan);
+    if ((threadIdx.x & 31) == 0) e.exps[(long long)r * act8_blocks(a.m) + (j >> 5)] = (uint8_t)byte;
+  }
+  if (!live) return;
+  v = act_value(e.act, v);
+  if (e.residual) v += ldg1((const T*)e.residual + r * e.ldr + j);
+  ((T*)e.out)[r * e.ldo + j] = Elem<T>::from_f(v);
+}
+
+// NT: groups of eight rows of x. MT: groups of 16 weight rows. VEC: rows of x and w can be read 16 bytes at a time.
+template <class T, int NT, int MT, bool VEC>
+__global__ void __launch_bounds__(32 * ROWS_WARPS) rows_mma_kernel(RowsArgs a) {
+  __shared__ float part[ROWS_WARPS][NT * 8][MT * 16 + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int m0 = blockIdx.x * 16 * MT;
+  const uint16_t* w0 = (const uint16_t*)a.w + (long long)(m0 + g) * a.ldw;
+  float acc[MT][NT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+  // warps take turns of 32 * U columns
+  constexpr int U = 4;
+  for (int k0 = warp * 32 * U; k0 < a.d; k0 += ROWS_WARPS * 32 * U) {
+    uint4 wq[MT][2][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          wq[m][h][u] = load16<VEC>(w0 + (long long)(16 * m + 8 * h) * a.ldw, k0 + u * 32 + t * 8, a.d, m0 + g + 16 * m + 8 * h < a.m);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = n * 8 + g;
+      const uint16_t* xr = (const uint16_t*)a.x + (long long)r * a.ldx;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint4 b = load16<VEC>(xr, k0 + u * 32 + t * 8, a.d, r < a.rows);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma_16816(acc[m][n], wq[m][0][u].x, wq[m][1][u].x, wq[m][0][u].y, wq[m][1][u].y, b.x, b.y, (const T*)nullptr);
+          mma_16816(acc[m][n], wq[m][0][u].z, wq[m][1][u].z, wq[m][0][u].w, wq[m][1][u].w, b.z, b.w, (const T*)nullptr);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // (weight row g or g + 8, token 2t or 2t + 1)
+        part[warp][n * 8 + 2 * t + (i & 1)][16 * m + g + 8 * (i >> 1)] = acc[m][n][i];
+  __syncthreads();
+  for (int r = warp; r < a.rows; r += ROWS_WARPS) {
+    const bool live = lane < MT * 16 && m0 + lane < a.m;
+    float v = 0.f;
+    if (live) {
+#pragma unroll
+      for (int w = 0; w < ROWS_WARPS; ++w) v += part[w][r][lane];
+    }
+    finish_element<T>(a, v, r, m0 + lane, live);
+  }
+}
+
+// float32: a warp takes two weight rows, lanes along the columns; a block 32.
+template <int NR, bool VEC>
+__global__ void __launch_bounds__(512) rows_f32_kernel(RowsArgs a) {
+  __shared__ float sums[NR][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m0 = blockIdx.x * 32 + warp * 2;
+  // rows past the end repeat the last one and are not stored
+  const float* w0 = (const float*)a.w + (long long)min(m0, a.m - 1) * a.ldw;
+  const float* w1 = (const float*)a.w + (long long)min(m0 + 1, a.m - 1) * a.ldw;
+  const float* x = (const float*)a.x;
+  float acc[2][NR];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < NR; ++r) acc[i][r] = 0.f;
+  if (VEC) {
+    constexpr int U = 4;
+    for (int k0 = lane * 4; k0 < a.d; k0 += 128 * U) {
+      float4 p[U], q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 128 * u;
+        p[u] = q[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < a.d) {
+          p[u] = __ldg(reinterpret_cast<const float4*>(w0 + k));
+          q[u] = __ldg(reinterpret_cast<const float4*>(w1 + k));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 128 * u;
+        if (k >= a.d) break;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          if (r < a.rows) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(x + r * a.ldx + k));
+            acc[0][r] = fmaf(p[u].x, v.x, fmaf(p[u].y, v.y, fmaf(p[u].z, v.z, fmaf(p[u].w, v.w, acc[0][r]))));
+            acc[1][r] = fmaf(q[u].x, v.x, fmaf(q[u].y, v.y, fmaf(q[u].z, v.z, fmaf(q[u].w, v.w, acc[1][r]))));
+          }
+        }
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (int k = lane; k < a.d; k += 32) {
+      const float p = __ldg(w0 + k), q = __ldg(w1 + k);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        if (r < a.rows) {
+          const float v = __ldg(x + r * a.ldx + k);
+          acc[0][r] = fmaf(p, v, acc[0][r]);
+          acc[1][r] = fmaf(q, v, acc[1][r]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float v = acc[i][r];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) sums[r][warp * 2 + i] = v;
+    }
+  __syncthreads();
+  if (warp < a.rows) {
+    const int j = blockIdx.x * 32 + lane;
+    finish_element<float>(a, sums[warp][lane], warp, j, j < a.m);
+  }
+}
+
+// Rows up to which the weight's bytes bound the product (16-bit: four 8-row
+// groups of mma.sync; float32: eight rows of multiply-adds).
+static bool few_rows(int dtype, long long rows) { return rows <= (dtype == SCMP_F32 ? 8 : 32); }
+
+static cudaError_t launch_rows(const void* x, long long ldx, const void* w, long long ldw, int rows, int d, int m,
+                               const Epilogue& e, int dtype, cudaStream_t st) {
+  const RowsArgs a{x, w, ldx, ldw, rows, d, m, e};
+  const size_t es = dtype_size(dtype);
+  const bool vec = rows_aligned16(x, ldx, es) && rows_aligned16(w, ldw, es) && (size_t)d * es % 16 == 0;
+  if (dtype == SCMP_F32) {
+    const int grid = cdiv(m, 32);
+    auto go = [&](auto nr) {
+      constexpr int NR = decltype(nr)::value;
+      if (vec)
+        rows_f32_kernel<NR, true><<<grid, 512, 0, st>>>(a);
+      else
+        rows_f32_kernel<NR, false><<<grid, 512, 0, st>>>(a);
+    };
+    if (rows <= 1) go(std::integral_constant<int, 1>{});
+    else if (rows <= 4) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 8>{});
+  } else {
+    // 32 weight rows per block halve x's reads; 16 fill the SMs with narrow layers (a
+    // checkpoint's blocks need 32). An element's sum is the same either way.
+    const int mt = e.codes || m >= 32 * 148 * 2 ? 2 : 1;
+    const int grid = cdiv(m, 16 * mt);
+    auto go = [&](auto* tag, auto nt) {
+      using T = std::remove_pointer_t<decltype(tag)>;
+      constexpr int NT = decltype(nt)::value;
+      if (mt == 2) {
+        if (vec)
+          rows_mma_kernel<T, NT, 2, true><<<grid, 32 * ROWS_WARPS, 0, st>>>(a);
+        else
+          rows_mma_kernel<T, NT, 2, false><<<grid, 32 * ROWS_WARPS, 0, st>>>(a);
+      } else {
+        if (vec)
+          rows_mma_kernel<T, NT, 1, true><<<grid, 32 * ROWS_WARPS, 0, st>>>(a);
+        else
+          rows_mma_kernel<T, NT, 1, false><<<grid, 32 * ROWS_WARPS, 0, st>>>(a);
+      }
+    };
+    auto type = [&](auto* tag) {
+      if (rows <= 8) go(tag, std::integral_constant<int, 1>{});
+      else if (rows <= 16) go(tag, std::integral_constant<int, 2>{});
+      else go(tag, std::integral_constant<int, 4>{});
+    };
+    if (dtype == SCMP_BF16) type((__nv_bfloat16*)nullptr);
+    else type((__half*)nullptr);
+  }
+  count_launch();
+  return cudaGetLastError();
+}
+
+}  // namespace lin
+}  // namespace scmp

@@ -450,26 +450,46 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Adds the partial tiles in order and runs the epilogue: a warp per 32 x 32 piece.
+// Adds the partial products in order and runs the epilogue: a lane per column
+// (32 columns are one block of an 8-bit checkpoint), JOIN_ROWS rows per warp at
+// a time so that their loads overlap.
+constexpr int JOIN_ROWS = 4;
 template <class T, bool FULL>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TcArgs g) {
-  __shared__ uint4 stg[4][256];
-  __shared__ __align__(16) float bias_s[4][32];
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs g) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row0 = (long long)(blockIdx.y * 4 + warp) * 32;
-  const int col0 = blockIdx.x * 32;
-  if (row0 >= g.m) return;  // whole warps
-  const int rows = (int)(g.m - row0 < 32 ? g.m - row0 : 32);
-  float v[32];
+  const long long row0 = ((long long)blockIdx.y * 8 + warp) * JOIN_ROWS;
+  const int col = blockIdx.x * 32 + lane;
+  const bool live = col < g.n;
+  const Epilogue& e = g.e;
+  float v[JOIN_ROWS];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = 0.f;
+  for (int r = 0; r < JOIN_ROWS; ++r) v[r] = 0.f;
+#pragma unroll 4
   for (int s = 0; s < g.splits; ++s) {
-    Stage<float>::load(stg[warp], lane, g.partial + (size_t)s * g.m * g.n, g.n, row0, rows, col0, g.n, g.n % 4 == 0);
-    __syncwarp();
-    Stage<float>::add_row(stg[warp], lane, v);
-    __syncwarp();
+    const float* p = g.partial + ((size_t)s * g.m + row0) * g.n + col;
+#pragma unroll
+    for (int r = 0; r < JOIN_ROWS; ++r)
+      if (live && row0 + r < g.m) v[r] += __ldg(p + (size_t)r * g.n);
   }
-  finish_piece<T, FULL>(g, v, stg[warp], bias_s[warp], lane, row0, rows, col0);
+  const float bias = FULL && e.bias && live ? (e.bias_f32 ? __ldg((const float*)e.bias + col) : ldg1((const T*)e.bias + col)) : 0.f;
+#pragma unroll
+  for (int r = 0; r < JOIN_ROWS; ++r) {
+    const long long row = row0 + r;
+    if (row >= g.m) break;  // whole warps
+    float y = v[r];
+    if (FULL) {
+      y += bias;
+      if (e.pre && live) ((T*)e.pre)[row * g.n + col] = Elem<T>::from_f(y);
+      if (e.codes) {
+        const uint32_t byte = act8_exponent(__reduce_max_sync(0xffffffffu, live ? __float_as_uint(y) & 0x7FFFFFFFu : 0u), act8_floor<T>());
+        if (live) e.codes[row * g.n + col] = (int8_t)act8_code(y, act8_inverse(byte), byte == kAct8Nan);
+        if (lane == 0) e.exps[row * act8_blocks(g.n) + blockIdx.x] = (uint8_t)byte;
+      }
+      y = act_value(e.act, y);
+      if (e.residual && live) y += ldg1((const T*)e.residual + row * e.ldr + col);
+    }
+    if (live) ((T*)e.out)[row * e.ldo + col] = Elem<T>::from_f(y);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -513,9 +533,11 @@ static bool make_map(CUtensorMap* map, const Operand& o, bool f16, int tile_rows
 struct Schedule {
   int bn, splits;
 };
-// Least estimated time, in SM clocks: waves of tiles over 74 SM pairs, a k block
-// at 2 clocks per tile column, 2500 per tile that nothing hides, and the
-// partial tiles' way through L2 and a second launch.
+// Least estimated time, in SM clocks: waves of tiles over 74 SM pairs; a k block
+// takes 560 clocks for 256 columns and 440 for 128 (32 and 24 KB per SM, at the
+// 55 to 58 bytes per clock that L2 delivers to an SM: measured 566 and 444 on
+// 4096 x 4096 x 11008); 2500 per tile that nothing hides; for a split product
+// the partial tiles' way through L2 and a second launch.
 static Schedule schedule_for(long long m, int n, long long kblocks) {
   Schedule best{256, 1};
   double least = 1e300;
@@ -524,8 +546,8 @@ static Schedule schedule_for(long long m, int n, long long kblocks) {
     const long long tiles = ((m + 255) / 256) * ((n + bn - 1) / bn);
     for (int s = 1; s <= 16 && (s == 1 || kblocks / s >= 4); ++s) {
       const long long waves = (tiles * s + pairs - 1) / pairs;
-      double t = waves * ((kblocks + s - 1) / s * 2.0 * bn + 2500.0);
-      if (s > 1) t += 6000.0 + (double)m * n * (s + 1) * 4 / 2500.0;
+      double t = waves * ((kblocks + s - 1) / s * (bn == 256 ? 560.0 : 440.0) + 2500.0);
+      if (s > 1) t += 5000.0 + (double)m * n * (s + 1) * 4 / 2500.0;
       if (t < least) {
         least = t;
         best = {bn, s};
@@ -561,7 +583,7 @@ static cudaError_t launch_tc_t(const CUtensorMap& ma, const CUtensorMap& mb, con
   e = cudaLaunchKernelEx(&cfg, kern, ma, mb, g);
   count_launch();
   if (e == cudaSuccess && g.splits > 1) {
-    join_kernel<T, FULL><<<dim3(cdiv(g.n, 32), (unsigned)((g.m + 127LL) / 128)), 128, 0, st>>>(g);
+    join_kernel<T, FULL><<<dim3(cdiv(g.n, 32), (unsigned)((g.m + 8LL * JOIN_ROWS - 1) / (8 * JOIN_ROWS))), 256, 0, st>>>(g);
     count_launch();
     e = cudaGetLastError();
   }

@@ -1,4 +1,5 @@
 // Translation unit of the exact linear layer.
+#include "linear_rows.cu"
 #include "linear_tc.cu"
 #include "linear.cu"
 
