@@ -65,43 +65,23 @@ class Act8:
         return f"Act8({tuple(self.shape)}, {self.dtype}, {self.device})"
 
 
-def _empty(shape, dtype: torch.dtype, device) -> Act8:
+def _wrap(codes: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype) -> Act8:
+    """An Act8 of tensors the library just wrote."""
     a = object.__new__(Act8)
-    a.codes = torch.empty(shape, dtype=torch.int8, device=device)
-    a.exponents = torch.empty((*shape[:-1], -(-shape[-1] // BLOCK)), dtype=torch.uint8, device=device)
-    a.dtype = dtype
+    a.codes, a.exponents, a.dtype = codes, exponents, dtype
     return a
 
 
-@torch.no_grad()
 def pack_act8(x: torch.Tensor) -> Act8:
     """The 8-bit checkpoint of ``x`` (..., cols), a float32, bfloat16 or float16
     CUDA tensor."""
-    dt = L.dtype_code("pack_act8", "x", x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"pack_act8: x needs a last axis, got shape {tuple(x.shape)}")
-    with L.on(x.device):
-        x2, rows, ld = L.rows_of(x)
-        a = _empty(x.shape, x.dtype, x.device)
-        L.call("scmp_act8_pack", x2.data_ptr(), dt, rows, x.shape[-1], ld, a.codes.data_ptr(), a.exponents.data_ptr(),
-               L.stream(x.device))
-    return a
+    return _wrap(*L.ext().act8_pack(x), x.dtype)
 
 
-@torch.no_grad()
 def unpack_act8(a: Act8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The values ``a`` stands for, as ``dtype`` (default: the packed tensor's).
     Exact, but that another dtype than the packed tensor's may round or overflow."""
-    dtype = a.dtype if dtype is None else dtype
-    if dtype not in L.DTYPES:
-        raise ValueError(f"unpack_act8: dtype must be float32, bfloat16 or float16, got {dtype}")
-    L.need_cuda("unpack_act8", "a", a.codes)
-    with L.on(a.device):
-        out = torch.empty(a.shape, dtype=dtype, device=a.device)
-        cols = a.shape[-1]
-        L.call("scmp_act8_unpack", a.codes.data_ptr(), a.exponents.data_ptr(), out.numel() // cols, cols, out.data_ptr(),
-               L.DTYPES[dtype], L.stream(a.device))
-    return out
+    return L.ext().act8_unpack(a.codes, a.exponents, a.dtype if dtype is None else dtype)
 
 
 __all__ = ["Act8", "pack_act8", "unpack_act8"]

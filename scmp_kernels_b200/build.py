@@ -1,4 +1,5 @@
-"""Build ``libscmp_b200.so`` from ``csrc/`` with nvcc for sm_100a.
+"""Build ``libscmp_b200.so`` from ``csrc/`` with nvcc for sm_100a, and the layers'
+Python binding ``_layers_ext.so`` beside it.
 
 Usage: ``python -m scmp_kernels_b200.build [--force]``. The library is built
 in the package directory so that it travels with the source tree.
@@ -15,6 +16,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
 OUT = os.path.join(HERE, "libscmp_b200.so")
+EXT = os.path.join(HERE, "_layers_ext.so")
+BINDING = os.path.join(HERE, "csrc", "binding.cpp")
 OBJ_DIR = os.path.join(HERE, "_build")
 
 # Translation units and the sources each depends on (file names in csrc/; the
@@ -46,10 +49,32 @@ def sources() -> list[str]:
 
 
 def up_to_date() -> bool:
-    if not os.path.exists(OUT):
+    if not os.path.exists(OUT) or not os.path.exists(EXT):
         return False
     t = os.path.getmtime(OUT)
-    return all(os.path.getmtime(s) <= t for s in sources())
+    return (all(os.path.getmtime(s) <= t for s in sources() if s != BINDING)
+            and os.path.getmtime(BINDING) <= os.path.getmtime(EXT))
+
+
+def _compile_binding(force: bool) -> None:
+    header = os.path.join(REPO, "include", "scmp_b200.h")
+    if not force and os.path.exists(EXT) and all(os.path.getmtime(f) <= os.path.getmtime(EXT) for f in (BINDING, header)):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    inc = [*include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include"), os.path.join(REPO, "include")]
+    cmd = ["g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in inc), BINDING, "-o", EXT,
+           f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           f"-L{HERE}", "-l:libscmp_b200.so", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"g++ failed ({r.returncode}): {' '.join(cmd)}")
 
 
 def _unit_sources(unit: str) -> list[str]:
@@ -89,6 +114,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         sys.stderr.write("".join(reports) + r.stdout + r.stderr)
     if r.returncode:
         raise RuntimeError(f"nvcc failed ({r.returncode}): {' '.join(cmd)}")
+    _compile_binding(force)
     return OUT
 
 

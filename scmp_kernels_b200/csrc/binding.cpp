@@ -1,0 +1,348 @@
+// Python binding of the layers: argument checks, outputs, workspaces and the
+// call into libscmp_b200.so, in C++ because a small layer's GPU time is below
+// what the same steps cost in Python (one 4096-wide token through
+// layer_norm_forward: 22 us per call from Python with ctypes, see norm.py for the
+// functions users call).
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <optional>
+#include <string>
+#include <tuple>
+
+#include "scmp_b200.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using Opt = std::optional<Tensor>;
+
+namespace {
+
+[[noreturn]] void refuse(const std::string& who, const std::string& what) { throw py::value_error(who + ": " + what); }
+
+// Status of a library call as the exception its kind maps to.
+void check(int status, const char* who) {
+  if (status == SCMP_OK) return;
+  std::string msg = scmp_last_error();
+  if (msg.find(who) == std::string::npos) msg = std::string(who) + ": " + msg;
+  if (status == SCMP_ERR_INVALID_ARG) throw py::value_error(msg);
+  if (status == SCMP_ERR_UNSUPPORTED) {
+    PyErr_SetString(PyExc_NotImplementedError, msg.c_str());
+    throw py::error_already_set();
+  }
+  throw std::runtime_error("scmp_kernels_b200 error " + std::to_string(status) + ": " + msg);
+}
+
+std::string name_of(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return "torch.float32";
+    case at::kBFloat16: return "torch.bfloat16";
+    case at::kHalf: return "torch.float16";
+    default: return c10::toString(t);
+  }
+}
+std::string str(c10::IntArrayRef s) {
+  std::string r = "(";
+  for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
+  return r + (s.size() == 1 ? ",)" : ")");
+}
+int code_of(at::ScalarType t) {
+  return t == at::kFloat ? SCMP_F32 : t == at::kBFloat16 ? SCMP_BF16 : t == at::kHalf ? SCMP_F16 : -1;
+}
+
+void need_cuda(const char* who, const char* name, const Tensor& t) {
+  if (t.is_cuda()) return;
+  if (c10::cuda::device_count() == 0)
+    throw std::runtime_error("scmp_kernels_b200: a CUDA device (B200, sm_100a) is required; this package has no CPU implementation");
+  refuse(who, std::string(name) + " must be a CUDA tensor, got one on " + t.device().str());
+}
+int dtype_code(const char* who, const char* name, const Tensor& t) {
+  const int c = code_of(t.scalar_type());
+  if (c < 0) refuse(who, std::string(name) + " must be float32, bfloat16 or float16, got " + name_of(t.scalar_type()));
+  need_cuda(who, name, t);
+  return c;
+}
+void need_last_axis(const char* who, const char* name, const Tensor& t) {
+  if (t.dim() < 1 || t.size(-1) < 1) refuse(who, std::string(name) + " needs a last axis, got shape " + str(t.sizes()));
+}
+void same_device(const char* who, const char* name, const Opt& t, const char* ref_name, const Tensor& ref) {
+  if (t && t->device() != ref.device())
+    refuse(who, std::string(name) + " is on " + t->device().str() + ", " + ref_name + " on " + ref.device().str());
+}
+int64_t leading(const Tensor& t) {
+  int64_t n = 1;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
+  return n;
+}
+bool same_leading(const Tensor& a, const Tensor& b) {
+  return a.dim() == b.dim() && a.sizes().slice(0, a.dim() - 1) == b.sizes().slice(0, b.dim() - 1);
+}
+
+// A tensor (..., cols) as rows at a fixed pitch, copied only where its strides
+// do not allow it.
+struct Rows {
+  Tensor t;
+  int64_t rows = 0, pitch = 0;
+  const void* p() const { return t.defined() ? t.const_data_ptr() : nullptr; }
+};
+Rows rows_of(const Tensor& t) {
+  const int64_t cols = t.size(-1), d = t.dim(), rows = leading(t);
+  if (t.is_contiguous()) return {t, rows, cols};
+  if (d > 1 && t.stride(-1) == 1 && t.stride(-2) >= cols) {
+    bool ok = true;
+    for (int64_t i = 0; i + 2 < d; ++i) ok = ok && t.stride(i) == t.stride(i + 1) * t.size(i + 1);
+    if (ok) return {t, rows, t.stride(-2)};
+  }
+  return {t.contiguous(), rows, cols};
+}
+
+// A vector of n values, float32 or of type `type`, contiguous.
+Tensor parameter(const char* who, const char* name, const Opt& p, at::ScalarType type, int64_t n) {
+  if (!p) return Tensor();
+  if (p->dim() != 1 || p->size(0) != n)
+    refuse(who, std::string(name) + " must be " + str({n}) + ", got " + str(p->sizes()));
+  if (p->scalar_type() != type && p->scalar_type() != at::kFloat)
+    refuse(who, std::string(name) + " must be float32 or " + name_of(type) + ", got " + name_of(p->scalar_type()));
+  return p->is_contiguous() ? *p : p->contiguous();
+}
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* mut(Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+template <class U>
+U* mut(Tensor& t) { return static_cast<U*>(mut(t)); }
+template <class U>
+const U* cptr(const Opt& t) { return t ? static_cast<const U*>(t->const_data_ptr()) : nullptr; }
+py::object obj(const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); }
+
+Tensor make(c10::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+  return at::empty(shape, like.options().dtype(type).requires_grad(false));
+}
+struct Packed {
+  Tensor codes, exps;
+};
+Packed make_packed(c10::IntArrayRef shape, const Tensor& like) {
+  c10::DimVector e(shape.begin(), shape.end());
+  e.back() = (e.back() + 31) / 32;
+  return {make(shape, at::kChar, like), make(e, at::kByte, like)};
+}
+c10::DimVector with_last(const Tensor& t, int64_t n) {
+  c10::DimVector s(t.sizes().begin(), t.sizes().end());
+  s.back() = n;
+  return s;
+}
+struct Workspace {
+  Tensor t;
+  size_t bytes;
+  void* p() { return mut(t); }
+};
+Workspace workspace(size_t bytes, const Tensor& like) {
+  return {bytes ? make({(int64_t)bytes}, at::kByte, like) : Tensor(), bytes};
+}
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// The library copies rows that do not start and step by 16 bytes; `flag` names
+// the operand.
+int unaligned(int flag, const Rows& r) {
+  if (!r.t.defined()) return 0;
+  return ((reinterpret_cast<uintptr_t>(r.p()) | (uintptr_t)(r.pitch * r.t.element_size())) & 15) ? flag : 0;
+}
+int narrow(const char* who, int64_t n) {
+  if (n > 2147480000) refuse(who, "an axis is too long: " + std::to_string(n));
+  return (int)n;
+}
+
+py::tuple act8_pack(const Tensor& x) {
+  const char* who = "pack_act8";
+  const int dt = dtype_code(who, "x", x);
+  need_last_axis(who, "x", x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Rows r = rows_of(x);
+  Packed p = make_packed(x.sizes(), x);
+  check(scmp_act8_pack(r.p(), dt, r.rows, narrow(who, x.size(-1)), r.pitch, mut<int8_t>(p.codes), mut<uint8_t>(p.exps), stream_of(x)), who);
+  return py::make_tuple(p.codes, p.exps);
+}
+
+Tensor act8_unpack(const Tensor& codes, const Tensor& exps, at::ScalarType type) {
+  const char* who = "unpack_act8";
+  if (code_of(type) < 0) refuse(who, "dtype must be float32, bfloat16 or float16, got " + name_of(type));
+  need_cuda(who, "a", codes);
+  const c10::cuda::CUDAGuard guard(codes.device());
+  Tensor out = make(codes.sizes(), type, codes);
+  check(scmp_act8_unpack((const int8_t*)codes.const_data_ptr(), (const uint8_t*)exps.const_data_ptr(), leading(codes),
+                         narrow(who, codes.size(-1)), mut(out), code_of(type), stream_of(codes)), who);
+  return out;
+}
+
+py::tuple layer_norm_forward(const Tensor& x, const Opt& weight, const Opt& bias, double eps, bool checkpoint8) {
+  const char* who = "layer_norm_forward";
+  const int dt = dtype_code(who, "x", x);
+  need_last_axis(who, "x", x);
+  const int64_t cols = x.size(-1);
+  const Tensor w = parameter(who, "weight", weight, x.scalar_type(), cols), b = parameter(who, "bias", bias, x.scalar_type(), cols);
+  if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
+    refuse(who, "weight and bias must have one dtype, got " + name_of(w.scalar_type()) + " and " + name_of(b.scalar_type()));
+  same_device(who, "weight", weight, "x", x);
+  same_device(who, "bias", bias, "x", x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Rows r = rows_of(x);
+  Tensor y = make(x.sizes(), x.scalar_type(), x);
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  Tensor mean = make(lead, at::kFloat, x), rstd = make(lead, at::kFloat, x);
+  Packed p;
+  if (checkpoint8) p = make_packed(x.sizes(), x);
+  const Tensor& param = w.defined() ? w : b;
+  check(scmp_layer_norm_forward(r.p(), dt, r.rows, narrow(who, cols), r.pitch, ptr(w), ptr(b),
+                                param.defined() ? code_of(param.scalar_type()) : dt, (float)eps, mut(y), mut<float>(mean),
+                                mut<float>(rstd), mut<int8_t>(p.codes), mut<uint8_t>(p.exps), stream_of(x)), who);
+  return checkpoint8 ? py::make_tuple(y, mean, rstd, p.codes, p.exps) : py::make_tuple(y, mean, rstd);
+}
+
+// x is a tensor, or the codes (with exps and type) of its checkpoint.
+py::tuple layer_norm_backward(const Tensor& dy, const Tensor& x, const Opt& exps, const std::optional<at::ScalarType>& packed_type,
+                              const Tensor& mean, const Tensor& rstd, const Opt& weight, bool with_bias) {
+  const char* who = "layer_norm_backward";
+  const int dt = dtype_code(who, "dy", dy);
+  const at::ScalarType x_type = exps ? *packed_type : x.scalar_type();
+  if (x.sizes() != dy.sizes()) refuse(who, "dy has shape " + str(dy.sizes()) + ", x " + str(x.sizes()));
+  need_last_axis(who, "dy", dy);
+  if (x_type != dy.scalar_type()) refuse(who, "dy is " + name_of(dy.scalar_type()) + ", x " + name_of(x_type));
+  const auto lead = dy.sizes().slice(0, dy.dim() - 1);
+  for (auto [name, s] : {std::pair<const char*, const Tensor*>{"mean", &mean}, {"rstd", &rstd}}) {
+    if (s->scalar_type() != at::kFloat || s->sizes() != lead)
+      refuse(who, std::string(name) + " must be float32 " + str(lead) + ", got " + name_of(s->scalar_type()) + " " + str(s->sizes()));
+    same_device(who, name, *s, "dy", dy);
+  }
+  const int64_t cols = dy.size(-1);
+  const Tensor w = parameter(who, "weight", weight, dy.scalar_type(), cols);
+  same_device(who, "x", x, "dy", dy);
+  same_device(who, "weight", weight, "dy", dy);
+  const c10::cuda::CUDAGuard guard(dy.device());
+  const Rows g = rows_of(dy), r = exps ? Rows{} : rows_of(x);
+  const Tensor mu = mean.contiguous(), rs = rstd.contiguous();
+  const at::ScalarType wtype = w.defined() ? w.scalar_type() : dy.scalar_type();
+  Tensor dx = make(dy.sizes(), dy.scalar_type(), dy), dw, db;
+  if (w.defined()) dw = make({cols}, wtype, dy);
+  if (with_bias) db = make({cols}, wtype, dy);
+  size_t bytes = 0;
+  if (w.defined() || with_bias) check(scmp_layer_norm_backward_workspace_size(g.rows, narrow(who, cols), &bytes), who);
+  Workspace ws = workspace(bytes, dy);
+  check(scmp_layer_norm_backward(g.p(), g.pitch, r.p(), r.pitch, exps ? (const int8_t*)x.const_data_ptr() : nullptr,
+                                 cptr<uint8_t>(exps), dt, g.rows, narrow(who, cols), (const float*)mu.const_data_ptr(),
+                                 (const float*)rs.const_data_ptr(), ptr(w), code_of(wtype), mut(dx), mut(dw), mut(db), ws.p(),
+                                 ws.bytes, stream_of(dy)), who);
+  return py::make_tuple(dx, obj(dw), obj(db));
+}
+
+void check_weight(const char* who, const Tensor& w, at::ScalarType type, int64_t d, int64_t m) {
+  if (w.dim() != 2) refuse(who, "weight must be 2D (M, D), got " + std::to_string(w.dim()) + "D");
+  if (w.scalar_type() != type) refuse(who, "weight is " + name_of(w.scalar_type()) + ", expected " + name_of(type));
+  if (w.size(0) < 1 || w.size(1) < 1) refuse(who, "weight has no values: " + str(w.sizes()));
+  if ((d >= 0 && w.size(1) != d) || (m >= 0 && w.size(0) != m))
+    refuse(who, "inner dimension mismatch: weight is " + str(w.sizes()) + ", expected (" + (m < 0 ? "M" : std::to_string(m)) +
+                    ", " + (d < 0 ? "D" : std::to_string(d)) + ")");
+}
+
+// save: 0 nothing, 1 the pre-activation, 2 its 8-bit checkpoint.
+py::object linear_forward(const Tensor& x, const Tensor& weight, const Opt& bias, int act, const Opt& residual, int save) {
+  const char* who = "linear_forward";
+  const int dt = dtype_code(who, "x", x);
+  need_last_axis(who, "x", x);
+  const int64_t d = x.size(-1);
+  check_weight(who, weight, x.scalar_type(), d, -1);
+  const int64_t m = weight.size(0);
+  const auto shape = with_last(x, m);
+  const Tensor b = parameter(who, "bias", bias, x.scalar_type(), m);
+  if (residual && (residual->scalar_type() != x.scalar_type() || residual->sizes() != c10::IntArrayRef(shape)))
+    refuse(who, "residual must be " + name_of(x.scalar_type()) + " " + str(shape) + ", got " + name_of(residual->scalar_type()) + " " + str(residual->sizes()));
+  same_device(who, "weight", weight, "x", x);
+  same_device(who, "bias", bias, "x", x);
+  same_device(who, "residual", residual, "x", x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Rows r = rows_of(x), w = rows_of(weight), res = residual ? rows_of(*residual) : Rows{};
+  Tensor y = make(shape, x.scalar_type(), x), pre;
+  Packed p;
+  if (save == 1) pre = make(shape, x.scalar_type(), x);
+  if (save == 2) p = make_packed(shape, x);
+  size_t bytes = 0;
+  const int di = narrow(who, d), mi = narrow(who, m);
+  check(scmp_linear_forward_workspace_size(dt, r.rows, di, mi, unaligned(1, r) | unaligned(2, w), &bytes), who);
+  Workspace ws = workspace(bytes, x);
+  check(scmp_linear_forward(r.p(), r.pitch, w.p(), w.pitch, ptr(b), b.defined() ? code_of(b.scalar_type()) : dt, res.p(), res.pitch,
+                            dt, r.rows, di, mi, act, mut(y), mut(pre), mut<int8_t>(p.codes), mut<uint8_t>(p.exps), ws.p(), ws.bytes,
+                            stream_of(x)), who);
+  if (save == 1) return py::make_tuple(y, pre);
+  if (save == 2) return py::make_tuple(y, p.codes, p.exps);
+  return py::cast(y);
+}
+
+// x and pre are tensors, or the codes (with exps and type) of their checkpoints.
+py::tuple linear_backward(const Tensor& dy, const Opt& x, const Opt& x_exps, const std::optional<at::ScalarType>& x_packed,
+                          const Opt& weight, int act, const Opt& pre, const Opt& pre_exps,
+                          const std::optional<at::ScalarType>& pre_packed, bool with_bias,
+                          const std::optional<at::ScalarType>& bias_dtype, bool need_dx, bool need_dweight) {
+  const char* who = "linear_backward";
+  const int dt = dtype_code(who, "dy", dy);
+  const at::ScalarType type = dy.scalar_type(), btype = bias_dtype.value_or(type);
+  need_last_axis(who, "dy", dy);
+  const int64_t m = dy.size(-1);
+  if (btype != type && btype != at::kFloat) refuse(who, "bias_dtype must be float32 or " + name_of(type) + ", got " + name_of(btype));
+  if (need_dx && !weight) refuse(who, "dx needs the weight");
+  if (need_dweight && !x) refuse(who, "dweight needs x");
+  int64_t d = -1;
+  if (x) {
+    const at::ScalarType xt = x_exps ? *x_packed : x->scalar_type();
+    if (xt != type) refuse(who, "dy is " + name_of(type) + ", x " + name_of(xt));
+    if (!same_leading(*x, dy) || x->size(-1) < 1) refuse(who, "dy has shape " + str(dy.sizes()) + ", x " + str(x->sizes()));
+    d = x->size(-1);
+  }
+  if (weight) {
+    check_weight(who, *weight, type, d, m);
+    d = weight->size(1);
+  }
+  const bool with_pre = act != SCMP_ACT_NONE;
+  if (with_pre) {
+    if (!pre) refuse(who, "the activation needs pre, the pre-activation");
+    const at::ScalarType pt = pre_exps ? *pre_packed : pre->scalar_type();
+    if (pt != type || pre->sizes() != dy.sizes())
+      refuse(who, "pre must be " + name_of(type) + " " + str(dy.sizes()) + ", got " + name_of(pt) + " " + str(pre->sizes()));
+    same_device(who, "pre", pre, "dy", dy);
+  }
+  same_device(who, "x", x, "dy", dy);
+  same_device(who, "weight", weight, "dy", dy);
+  const int parts = (need_dx ? 1 : 0) | (need_dweight ? 2 : 0) | (with_bias ? 4 : 0);
+  if (!parts) return py::make_tuple(py::none(), py::none(), py::none());
+  const c10::cuda::CUDAGuard guard(dy.device());
+  const bool x8 = need_dweight && x_exps, p8 = with_pre && pre_exps;
+  const Rows g = rows_of(dy), r = need_dweight && !x8 ? rows_of(*x) : Rows{}, w = need_dx ? rows_of(*weight) : Rows{},
+             p = with_pre && !p8 ? rows_of(*pre) : Rows{};
+  Tensor dx, dw, db;
+  if (need_dx) dx = make(with_last(dy, d), type, dy);
+  if (need_dweight) dw = make({m, d}, type, dy);
+  if (with_bias) db = make({m}, btype, dy);
+  const int di = narrow(who, d < 1 ? 1 : d), mi = narrow(who, m);
+  size_t bytes = 0;
+  check(scmp_linear_backward_workspace_size(dt, g.rows, di, mi, act, x8, parts, unaligned(4, g) | unaligned(1, r) | unaligned(2, w), &bytes), who);
+  Workspace ws = workspace(bytes, dy);
+  check(scmp_linear_backward(g.p(), g.pitch, r.p(), r.pitch, x8 ? cptr<int8_t>(x) : nullptr, x8 ? cptr<uint8_t>(x_exps) : nullptr,
+                             w.p(), w.pitch, p.p(), p.pitch, p8 ? cptr<int8_t>(pre) : nullptr, p8 ? cptr<uint8_t>(pre_exps) : nullptr,
+                             dt, g.rows, di, mi, act, mut(dx), mut(dw), mut(db), code_of(btype), ws.p(), ws.bytes, stream_of(dy)), who);
+  return py::make_tuple(obj(dx), obj(dw), obj(db));
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_layers_ext, m) {
+  m.def("act8_pack", &act8_pack);
+  m.def("act8_unpack", &act8_unpack);
+  m.def("layer_norm_forward", &layer_norm_forward);
+  m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("linear_forward", &linear_forward);
+  m.def("linear_backward", &linear_backward);
+  m.def("rows_of", [](const Tensor& t) {
+    const Rows r = rows_of(t);
+    return std::make_tuple(r.t, r.rows, r.pitch);
+  });
+}

@@ -18,7 +18,7 @@ import torch
 
 from . import _layers as L
 from . import _lib
-from .act8 import Act8, _empty
+from .act8 import Act8, _wrap, pack_act8
 
 
 def _activation(who: str, activation) -> int:
@@ -29,19 +29,9 @@ def _activation(who: str, activation) -> int:
     return code
 
 
-def _weight(who: str, weight: torch.Tensor, dtype: torch.dtype, d: Optional[int], m: Optional[int]):
-    if weight.dim() != 2:
-        raise ValueError(f"{who}: weight must be 2D (M, D), got {weight.dim()}D")
-    if weight.dtype != dtype:
-        raise ValueError(f"{who}: weight is {weight.dtype}, expected {dtype}")
-    if weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"{who}: weight has no values: {tuple(weight.shape)}")
-    if (d is not None and weight.shape[1] != d) or (m is not None and weight.shape[0] != m):
-        raise ValueError(f"{who}: inner dimension mismatch: weight is {tuple(weight.shape)}, "
-                         f"expected ({'M' if m is None else m}, {'D' if d is None else d})")
+_SAVE = {None: 0, "exact": 1, "8bit": 2}
 
 
-@torch.no_grad()
 def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
                    activation: Optional[str] = None, residual: Optional[torch.Tensor] = None,
                    save: Optional[str] = None):
@@ -51,39 +41,13 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     also returns the pre-activation ``x @ weight.T + bias`` (x's dtype), "8bit" its
     :class:`Act8`, written by the same pass: ``(y, pre)`` instead of ``y``.
     """
-    who = "linear_forward"
-    dt = L.dtype_code(who, "x", x)
-    act = _activation(who, activation)
-    if save not in (None, "exact", "8bit"):
-        raise ValueError(f"{who}: unknown save '{save}'. Expected None, 'exact' or '8bit'.")
-    if x.dim() < 1:
-        raise ValueError(f"{who}: x needs a last axis")
-    d = x.shape[-1]
-    _weight(who, weight, x.dtype, d, None)
-    m = weight.shape[0]
-    shape = (*x.shape[:-1], m)
-    bias = L.parameter(who, "bias", bias, x.dtype, m)
-    if residual is not None and (residual.dtype != x.dtype or tuple(residual.shape) != shape):
-        raise ValueError(f"{who}: residual must be {x.dtype} {shape}, got {residual.dtype} {tuple(residual.shape)}")
-    L.same_place(who, x, weight=weight, bias=bias, residual=residual)
-    dev = x.device
-    with L.on(dev):
-        x2, rows, ldx = L.rows_of(x)
-        w2, _, ldw = L.rows_of(weight)
-        r2, _, ldr = (None, 0, 0) if residual is None else L.rows_of(residual)
-        y = torch.empty(shape, dtype=x.dtype, device=dev)
-        pre = torch.empty(shape, dtype=x.dtype, device=dev) if save == "exact" else \
-            _empty(shape, x.dtype, dev) if save == "8bit" else None
-        ws, nbytes, keep = L.workspace(dev, "scmp_linear_forward_workspace_size", dt, rows, d, m,
-                                       L.unaligned(1, x2, ldx) | L.unaligned(2, w2, ldw))
-        L.call("scmp_linear_forward", x2.data_ptr(), ldx, w2.data_ptr(), ldw, L.ptr(bias),
-               dt if bias is None else L.DTYPES[bias.dtype], L.ptr(r2), ldr, dt, rows, d, m, act, y.data_ptr(),
-               pre.data_ptr() if save == "exact" else None, pre.codes.data_ptr() if save == "8bit" else None,
-               pre.exponents.data_ptr() if save == "8bit" else None, ws, nbytes, L.stream(dev))
-    return y if save is None else (y, pre)
+    act = _activation("linear_forward", activation)
+    if save not in _SAVE:
+        raise ValueError(f"linear_forward: unknown save '{save}'. Expected None, 'exact' or '8bit'.")
+    out = L.ext().linear_forward(x, weight, bias, act, residual, _SAVE[save])
+    return (out[0], _wrap(out[1], out[2], x.dtype)) if save == "8bit" else out
 
 
-@torch.no_grad()
 def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Act8, None], weight: Optional[torch.Tensor], *,
                     activation: Optional[str] = None, pre: Union[torch.Tensor, Act8, None] = None,
                     with_bias: bool = True, bias_dtype: Optional[torch.dtype] = None, need_dx: bool = True,
@@ -98,61 +62,13 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Act8, None], weight
     products share is rounded to dy's dtype once; dbias is summed before that
     rounding.
     """
-    who = "linear_backward"
-    dt = L.dtype_code(who, "dy", dy)
-    act = _activation(who, activation)
-    if dy.dim() < 1 or dy.shape[-1] < 1:
-        raise ValueError(f"{who}: dy needs a last axis, got shape {tuple(dy.shape)}")
-    m, lead, dev = dy.shape[-1], tuple(dy.shape[:-1]), dy.device
-    bias_dtype = dy.dtype if bias_dtype is None else bias_dtype
-    if bias_dtype != dy.dtype and bias_dtype != torch.float32:
-        raise ValueError(f"{who}: bias_dtype must be float32 or {dy.dtype}, got {bias_dtype}")
-    if need_dx and weight is None:
-        raise ValueError(f"{who}: dx needs the weight")
-    if need_dweight and x is None:
-        raise ValueError(f"{who}: dweight needs x")
-    d = None
-    if x is not None:
-        if x.dtype != dy.dtype:
-            raise ValueError(f"{who}: dy is {dy.dtype}, x {x.dtype}")
-        if tuple(x.shape[:-1]) != lead or x.shape[-1] < 1:
-            raise ValueError(f"{who}: dy has shape {tuple(dy.shape)}, x {tuple(x.shape)}")
-        d = x.shape[-1]
-    if weight is not None:
-        _weight(who, weight, dy.dtype, d, m)
-        d = weight.shape[1]
-    if act:
-        if pre is None:
-            raise ValueError(f"{who}: activation '{activation}' needs pre, the pre-activation")
-        if pre.dtype != dy.dtype or tuple(pre.shape) != tuple(dy.shape):
-            raise ValueError(f"{who}: pre must be {dy.dtype} {tuple(dy.shape)}, got {pre.dtype} {tuple(pre.shape)}")
-    else:
-        pre = None
-    for name, t in (("x", x), ("weight", weight), ("pre", pre)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{who}: {name} is on {t.device}, dy on {dev}")
-    x8 = x if isinstance(x, Act8) and need_dweight else None
-    p8 = pre if isinstance(pre, Act8) else None
-    with L.on(dev):
-        dy2, rows, ldy = L.rows_of(dy)
-        x2, _, ldx = L.rows_of(x) if need_dweight and x8 is None else (None, 0, 0)
-        w2, _, ldw = L.rows_of(weight) if need_dx else (None, 0, 0)
-        p2, _, ldp = L.rows_of(pre) if pre is not None and p8 is None else (None, 0, 0)
-        dx = torch.empty((*lead, d), dtype=dy.dtype, device=dev) if need_dx else None
-        dw = torch.empty((m, d), dtype=dy.dtype, device=dev) if need_dweight else None
-        db = torch.empty(m, dtype=bias_dtype, device=dev) if with_bias else None
-        parts = int(need_dx) | 2 * int(need_dweight) | 4 * int(with_bias)
-        if not parts:
-            return None, None, None
-        d = 1 if d is None else d
-        ws, nbytes, keep = L.workspace(dev, "scmp_linear_backward_workspace_size", dt, rows, d, m, act,
-                                       int(x8 is not None), parts,
-                                       L.unaligned(4, dy2, ldy) | L.unaligned(1, x2, ldx) | L.unaligned(2, w2, ldw))
-        L.call("scmp_linear_backward", dy2.data_ptr(), ldy, L.ptr(x2), ldx, x8.codes.data_ptr() if x8 is not None else None,
-               x8.exponents.data_ptr() if x8 is not None else None, L.ptr(w2), ldw, L.ptr(p2), ldp,
-               p8.codes.data_ptr() if p8 is not None else None, p8.exponents.data_ptr() if p8 is not None else None, dt,
-               rows, d, m, act, L.ptr(dx), L.ptr(dw), L.ptr(db), L.DTYPES[bias_dtype], ws, nbytes, L.stream(dev))
-    return dx, dw, db
+    act = _activation("linear_backward", activation)
+    x8 = p8 = xe = pe = None
+    if isinstance(x, Act8):
+        x, xe, x8 = x.codes, x.exponents, x.dtype
+    if isinstance(pre, Act8):
+        pre, pe, p8 = pre.codes, pre.exponents, pre.dtype
+    return L.ext().linear_backward(dy, x, xe, x8, weight, act, pre, pe, p8, with_bias, bias_dtype, need_dx, need_dweight)
 
 
 class _Linear(torch.autograd.Function):
@@ -168,7 +84,6 @@ class _Linear(torch.autograd.Function):
         if not need_w:
             kept += [None, None]
         elif eight:
-            from .act8 import pack_act8
             x8 = pack_act8(x)
             kept += [x8.codes, x8.exponents]
         else:

@@ -93,7 +93,7 @@ def test_rows_of_keeps_what_strides_allow():
                                    (t.t(), 60, 4, False), (t.view(2, 2, 60)[..., 1:9], 4, 60, True),
                                    (t.view(2, 2, 60)[:, :1], 2, 60, False), (t[:, ::2], 4, 30, False),
                                    (t[0], 1, 60, True), (t[:1].expand(4, 60), 4, 60, False)]:
-        u, r, p = _layers.rows_of(v)
+        u, r, p = _layers.ext().rows_of(v)
         assert (r, p) == (rows, pitch) and (u.data_ptr() == v.data_ptr()) == shares
         flat = torch.as_strided(u, (r, v.shape[-1]), (p, 1), u.storage_offset())
         assert torch.equal(flat, v.reshape(r, v.shape[-1]))
