@@ -39,9 +39,8 @@ __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x,
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const uint32_t byte = act8_exponent(top, act8_floor<T>());
     const float inv = act8_inverse(byte);
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)(act8_code(v[i], inv, byte == kAct8Nan) & 0xFF) << (8 * (i & 3));
+    const bool nan = byte == kAct8Nan;
+    const uint32_t w[2] = {act8_codes4(v[0], v[1], v[2], v[3], inv, nan), act8_codes4(v[4], v[5], v[6], v[7], inv, nan)};
     if (!live) continue;
     int8_t* dst = codes + row * cols + c0;
     if (VEC) {
@@ -73,7 +72,7 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const int8_t* __restri
       const uint2 q = __ldg(reinterpret_cast<const uint2*>(src));
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmul((float)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3))), s);
+      for (int i = 0; i < 8; ++i) v[i] = act8_value(i < 4 ? q.x : q.y, i & 3, s);
       stg8(dst, v);
     } else {
 #pragma unroll

@@ -42,9 +42,26 @@ __device__ __forceinline__ float act8_inverse(uint32_t byte) {
 __device__ __forceinline__ float act8_scale(uint32_t byte) {
   return byte == kAct8Nan ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte << 23);
 }
+// Adding 1.5 * 2^23 rounds to an integer, half to even, in the low bits.
+__device__ __forceinline__ uint32_t act8_rounded(float x, float inverse) {
+  const float magic = 12582912.f;
+  return __float_as_uint(fminf(fmaxf(fmaf(x, inverse, magic), magic - 127.f), magic + 127.f));
+}
 __device__ __forceinline__ int act8_code(float x, float inverse, bool nan_block) {
-  const int c = __float2int_rn(fclamp(fmul(x, inverse), -127.f, 127.f));
-  return nan_block ? 0 : c;
+  return nan_block ? 0 : (int)(int8_t)(act8_rounded(x, inverse) & 0xFFu);
+}
+// Four codes as the bytes of a word.
+__device__ __forceinline__ uint32_t act8_codes4(float a, float b, float c, float d, float inverse, bool nan_block) {
+  const uint32_t lo = __byte_perm(act8_rounded(a, inverse), act8_rounded(b, inverse), 0x0040);
+  const uint32_t hi = __byte_perm(act8_rounded(c, inverse), act8_rounded(d, inverse), 0x0040);
+  return nan_block ? 0u : __byte_perm(lo, hi, 0x5410);
+}
+// The value of byte i of a word of codes: the byte (offset by 128) becomes the
+// low mantissa bits of 2^23, which is then subtracted. Conversions from
+// integers would share the pipe of exp2 and reciprocal.
+__device__ __forceinline__ float act8_value(uint32_t codes, int i, float scale) {
+  const uint32_t u = __byte_perm(codes ^ 0x80808080u, 0x4B000000u, 0x7650 | i);
+  return fmul(fsub(__uint_as_float(u), 8388736.f), scale);
 }
 
 // The values of a checkpoint as rows of type dtype at a pitch of ldo (act8.cu).

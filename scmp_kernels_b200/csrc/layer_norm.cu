@@ -76,7 +76,7 @@ __device__ __forceinline__ void load_chunk8(const int8_t* __restrict__ codes, co
       const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes + c));
       const float s = act8_scale(__ldg(exps + (c >> 5)));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fmul((float)(int8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3))), s);
+      for (int j = 0; j < 8; ++j) v[j] = act8_value(j < 4 ? q.x : q.y, j & 3, s);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = 0.f;
@@ -161,10 +161,9 @@ __device__ __forceinline__ void store_act8(int8_t* __restrict__ codes, uint8_t* 
     const float inv = act8_inverse(byte);
     const int c = (t + TPR * i) * 8;
     if (!live || c >= cols) return;
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j >> 2] |= (uint32_t)(act8_code(v[j], inv, byte == kAct8Nan) & 0xFF) << (8 * (j & 3));
-    *reinterpret_cast<uint2*>(codes + c) = make_uint2(w[0], w[1]);
+    const bool nan = byte == kAct8Nan;
+    *reinterpret_cast<uint2*>(codes + c) =
+        make_uint2(act8_codes4(v[0], v[1], v[2], v[3], inv, nan), act8_codes4(v[4], v[5], v[6], v[7], inv, nan));
     if ((t & 3) == 0) exps[c >> 5] = (uint8_t)byte;
   } else {
 #pragma unroll

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
           if (a.codes) {
             const float sc = act8_scale(cur.ex);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = fmul((float)(int8_t)((j < 4 ? cur.codes.x : cur.codes.y) >> (8 * (j & 3))), sc);
+            for (int j = 0; j < 8; ++j) p[j] = act8_value(j < 4 ? cur.codes.x : cur.codes.y, j & 3, sc);
           } else {
             unpack8(cur.pre, p);
           }
@@ -201,7 +201,7 @@ static ForwardPlan plan_forward(Carve& c, int dtype, long long rows, int d, int 
   const bool f32 = dtype == SCMP_F32;
   if (f32 || (unal & kUnalignedX)) p.x = c.take<char>(staged_bytes(dtype, rows, d));
   if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(dtype, m, d));
-  p.partial = c.take<char>(partial_bytes(rows, m, (d + KB - 1LL) / KB * (f32 ? 6 : 1)));
+  p.partial = c.take<char>(partial_bytes(rows, m, cdiv(d, KB), f32 ? 6 : 1));
   return p;
 }
 struct BackwardPlan {
@@ -224,11 +224,11 @@ static BackwardPlan plan_backward(Carve& c, int dtype, long long rows, int d, in
       p.x = c.take<char>(staged_bytes(SCMP_BF16, rows, d));
     else if (f32 || (unal & kUnalignedX))
       p.x = c.take<char>(staged_bytes(dtype, rows, d));
-    partial = partial_bytes(m, d, (rows + KB - 1) / KB * (f32 ? (x8 ? 3 : 6) : 1));
+    partial = partial_bytes(m, d, (int)((rows + KB - 1) / KB), f32 ? (x8 ? 3 : 6) : 1);
   }
   if (parts & 1) {
     if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(dtype, m, d));
-    const size_t q = partial_bytes(rows, d, (m + KB - 1LL) / KB * (f32 ? 6 : 1));
+    const size_t q = partial_bytes(rows, d, cdiv(m, KB), f32 ? 6 : 1);
     if (q > partial) partial = q;
   }
   p.partial = c.take<char>(partial);

@@ -10,8 +10,18 @@ namespace scmp {
 namespace lin {
 
 // The activations are evaluated for every element of a large product, so they
-// use the hardware's exp2 and reciprocal (a few 2^-23 relative each).
-__device__ __forceinline__ float reciprocal(float x) { return __fdividef(1.f, x); }
+// use the hardware's exp2 and reciprocal (a few 2^-23 relative each; results
+// below 2^-126 are zero).
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // Phi(-z) = erfc(z / sqrt 2) / 2 for z >= 0, and e = exp(-z^2 / 2):
 // exp(z^2 / 2) Phi(-z) as a polynomial in t = 1 / (1 + 0.3 z), least relative
@@ -27,13 +37,13 @@ __device__ __forceinline__ float normal_tail(float z, float& e) {
   p = fmaf(p, t, 0.09991350769996643f);
   p = fmaf(p, t, 0.1207539513707161f);
   p = fmaf(p, t, 0.11962930113077164f);
-  e = __expf(-0.5f * z * z);
+  e = exp2_fast(-0.72134752044448170f * z * z);
   return p * t * e;
 }
-__device__ __forceinline__ float sigmoid(float v) { return reciprocal(1.f + __expf(-v)); }
+__device__ __forceinline__ float sigmoid(float v) { return reciprocal(1.f + exp2_fast(-1.4426950408889634f * v)); }
 // exp(-v), finite: 1 - sigmoid(v) = exp(-v) sigmoid(v) keeps its digits where
 // sigmoid(v) is near 1.
-__device__ __forceinline__ float exp_minus(float v) { return __expf(fminf(-v, 80.f)); }
+__device__ __forceinline__ float exp_minus(float v) { return exp2_fast(fminf(-1.4426950408889634f * v, 115.f)); }
 // 0.5 (1 + tanh u) = sigmoid(2 u)
 __device__ __forceinline__ float gelu_tanh_arg(float v) { return 1.5957691216057308f * fmaf(0.044715f * v * v, v, v); }
 

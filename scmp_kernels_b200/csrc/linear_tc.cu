@@ -16,9 +16,15 @@
 // six plane pairs whose product can reach float32's last bit, smallest first,
 // in the same loop over k blocks. Dropped pairs are below 2^-24 of |a||b|.
 //
-// Few output tiles for the SMs: the k blocks are split over several clusters,
-// which leave float32 partial tiles that a second kernel adds in order and
-// runs the epilogue on.
+// Long sums (PROMOTE: every forward pass, and float32): the tensor core truncates
+// as it accumulates, a bias that grows with the length of the chain (1.4e-8
+// relative per 16 k values, measured); so a chain is cut every 512 k values
+// (float32: 256), and the epilogue warps add the pieces in registers with
+// rounding while the MMAs fill the other accumulator.
+//
+// The last wave, when its tiles do not fill the SMs: their k blocks are split
+// over several clusters, which leave float32 partial tiles that a second kernel
+// adds in order and runs the epilogue on.
 //
 // Every wait is bounded (common.cuh): on a timeout the kernel records
 // SCMP_ERR_TIMEOUT and all roles leave.
@@ -36,15 +42,16 @@ constexpr int TC_THREADS = 128 + 32 * EPI_WARPS;
 constexpr int ACC_COLS = 256;     // tensor-memory columns between the two accumulators
 constexpr int MAX_SEGMENTS = 6;
 
-template <int BN>
+template <class T, int BN>
 struct Cfg {
   static constexpr int A_BYTES = 128 * KB * 2;
   static constexpr int B_BYTES = BN / 2 * KB * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 6 : 8;
-  static constexpr int STG = EPI_WARPS * 4096;  // 32 rows x 128 bytes per epilogue warp
-  static constexpr int BIAS = EPI_WARPS * 128;
-  static constexpr int SMEM = STAGES * STAGE + STG + BIAS + 256 + 1024;
+  static constexpr int PIECE = 32 * 32 * sizeof(T);          // a 32 x 32 piece of the result
+  static constexpr int STG = EPI_WARPS * 2 * PIECE;          // per epilogue warp: result and residual
+  static constexpr int STAGES = BN == 256 ? (sizeof(T) == 4 ? 5 : 6) : (sizeof(T) == 4 ? 6 : 8);
+  static constexpr int NP = BN / 64;            // 32-column pieces per epilogue warp
+  static constexpr int SMEM = STAGES * STAGE + STG + 512 + 1024;
 };
 
 struct TcArgs {
@@ -52,10 +59,13 @@ struct TcArgs {
   int kblocks;           // k blocks of one plane pair
   int segments;          // plane pairs
   uint8_t pa[MAX_SEGMENTS], pb[MAX_SEGMENTS];
-  int tiles_m, tiles_n, splits;
+  int chunk;             // k blocks per accumulator chain (PROMOTE), of every plane pair
+  int tiles_m, tiles_n;
+  int whole, splits;     // tiles run whole; the others in `splits` parts each
   int f16;               // operands are float16, else bfloat16
-  int vec_out, vec_res, vec_pre, vec_codes;  // rows can be accessed 16 bytes at a time
-  float* partial;        // (splits, m, n), or null
+  int tma_out, tma_res, tma_pre;  // the tensor can be accessed by TMA (16-byte base and pitch)
+  int vec_codes;                  // rows of codes can be written 16 bytes at a time
+  float* partial;        // (tiles - whole, splits, 256, BN)
   Epilogue e;
 };
 
@@ -113,26 +123,41 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr));
 }
 
-template <class F>
-__device__ __forceinline__ void act_each(float (&v)[32], F&& f) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = f(v[j]);
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
 }
-__device__ __forceinline__ void act_values(int act, float (&v)[32]) {
-  if (act == SCMP_ACT_RELU) act_each(v, [](float x) { return act_value(SCMP_ACT_RELU, x); });
-  if (act == SCMP_ACT_GELU) act_each(v, [](float x) { return act_value(SCMP_ACT_GELU, x); });
-  if (act == SCMP_ACT_GELU_TANH) act_each(v, [](float x) { return act_value(SCMP_ACT_GELU_TANH, x); });
-  if (act == SCMP_ACT_SILU) act_each(v, [](float x) { return act_value(SCMP_ACT_SILU, x); });
-}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// A warp's 32 rows x 32 columns between registers (a row per lane) and memory,
-// through a 4 KB staging area: 16-byte pieces, the piece index of a row
-// exclusive-ored so that neither side has bank conflicts; memory is accessed in
-// whole row segments of 64 (16-bit) or 128 bytes.
+// The tensor maps of a product: operands, and the epilogue's tensors as 32 x 32
+// boxes in the layout of Piece.
+struct Maps {
+  CUtensorMap a, b, out, pre, res;
+};
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// This thread's stores have read shared memory.
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+      "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A 32 x 32 piece in shared memory: rows of 64 (16-bit) or 128 bytes, the 16-byte
+// pieces of a row exclusive-ored as TMA's 64- and 128-byte swizzles do, so that
+// neither a row per lane nor a row segment per store has bank conflicts.
 template <class T>
-struct Stage {
-  static constexpr int PIECES = 32 * sizeof(T) / 16;  // 16-byte pieces per row: 4 or 8
-  static constexpr int PER = 16 / sizeof(T);          // values per piece
+struct Piece {
+  static constexpr int PIECES = 32 * sizeof(T) / 16, PER = 16 / sizeof(T);
   static __device__ __forceinline__ int slot(int row, int piece) {
     return row * PIECES + (piece ^ (PIECES == 4 ? (row >> 1) & 3 : row & 7));
   }
@@ -140,9 +165,13 @@ struct Stage {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       uint4 q;
-      T* e = reinterpret_cast<T*>(&q);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) e[i] = Elem<T>::from_f(v[p * PER + i]);
+      if constexpr (sizeof(T) == 2) {
+        const T* t = nullptr;
+        q = make_uint4(pack2(v[8 * p], v[8 * p + 1], t), pack2(v[8 * p + 2], v[8 * p + 3], t), pack2(v[8 * p + 4], v[8 * p + 5], t),
+                       pack2(v[8 * p + 6], v[8 * p + 7], t));
+      } else {
+        q = make_uint4(__float_as_uint(v[4 * p]), __float_as_uint(v[4 * p + 1]), __float_as_uint(v[4 * p + 2]), __float_as_uint(v[4 * p + 3]));
+      }
       s[slot(lane, p)] = q;
     }
   }
@@ -155,120 +184,161 @@ struct Stage {
       for (int i = 0; i < PER; ++i) v[p * PER + i] += Elem<T>::to_f(e[i]);
     }
   }
-  // staging -> rows row0.. of a matrix, columns col0..col0+31
-  static __device__ __forceinline__ void store(const uint4* s, int lane, T* base, long long ld, long long row0, int rows,
-                                               int col0, int cols, bool vec) {
-    if (vec && col0 + 32 <= cols) {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int row = i * (32 / PIECES) + lane / PIECES, p = lane % PIECES;
-        if (row < rows) *reinterpret_cast<uint4*>(base + (row0 + row) * ld + col0 + p * PER) = s[slot(row, p)];
-      }
-    } else {
-      const int c = lane;
-      for (int row = 0; row < rows; ++row) {
-        const T e = reinterpret_cast<const T*>(s + slot(row, c / PER))[c % PER];
-        if (col0 + c < cols) base[(row0 + row) * ld + col0 + c] = e;
-      }
-    }
+  // Tensors that TMA cannot access: a lane per column, row after row.
+  static __device__ __forceinline__ void store_rows(const uint4* s, int lane, T* base, long long ld, long long row0, int rows, int col0,
+                                                    int cols) {
+    if (col0 + lane >= cols) return;
+    T* p = base + row0 * ld + col0 + lane;
+#pragma unroll 4
+    for (int row = 0; row < rows; ++row) p[row * ld] = reinterpret_cast<const T*>(s + slot(row, lane / PER))[lane % PER];
   }
-  static __device__ __forceinline__ void load(uint4* s, int lane, const T* base, long long ld, long long row0, int rows,
-                                              int col0, int cols, bool vec) {
-    if (vec && col0 + 32 <= cols) {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int row = i * (32 / PIECES) + lane / PIECES, p = lane % PIECES;
-        if (row < rows) s[slot(row, p)] = __ldg(reinterpret_cast<const uint4*>(base + (row0 + row) * ld + col0 + p * PER));
-      }
-    } else {
-      const int c = lane;
-      for (int row = 0; row < rows; ++row)
-        reinterpret_cast<T*>(s + slot(row, c / PER))[c % PER] = col0 + c < cols ? base[(row0 + row) * ld + col0 + c] : T(0.f);
-    }
+  static __device__ __forceinline__ void load_rows(uint4* s, int lane, const T* base, long long ld, long long row0, int rows, int col0,
+                                                   int cols) {
+    if (col0 + lane >= cols) return;
+    const T* p = base + row0 * ld + col0 + lane;
+#pragma unroll 8
+    for (int row = 0; row < rows; ++row) reinterpret_cast<T*>(s + slot(row, lane / PER))[lane % PER] = p[row * ld];
   }
 };
 
-// Bias, checkpoint, activation, residual and stores of a warp's 32 x 32 piece
-// (a row per lane in v).
-template <class T, bool FULL>
-__device__ __forceinline__ void finish_piece(const TcArgs& g, float (&v)[32], uint4* stg, float* bias_s, int lane,
-                                             long long row0, int rows, int col0) {
-  using S = Stage<T>;
-  const Epilogue& e = g.e;
-  if (FULL) {
-    if (e.bias) {
-      const int c = col0 + lane;
-      bias_s[lane] = c >= g.n ? 0.f : e.bias_f32 ? __ldg((const float*)e.bias + c) : ldg1((const T*)e.bias + c);
-      __syncwarp();
+template <int ACT>
+__device__ __forceinline__ void act_all(float (&v)[32]) {
 #pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        const float4 b = reinterpret_cast<const float4*>(bias_s)[p];
-        v[4 * p] += b.x;
-        v[4 * p + 1] += b.y;
-        v[4 * p + 2] += b.z;
-        v[4 * p + 3] += b.w;
-      }
-    }
+  for (int j = 0; j < 32; ++j) v[j] = act_value(ACT, v[j]);
+}
+
+// An epilogue warp's shared memory: a piece of the result, a piece of the
+// residual and the barrier of the residual's loads.
+struct WarpStage {
+  uint4* out;
+  uint4* res;
+  uint32_t bar;
+  uint32_t phase;
+};
+// Starts the load of a piece of the residual (one lane).
+template <class T>
+__device__ __forceinline__ void start_residual(const Maps& maps, const WarpStage& w, long long row0, int col0) {
+  expect_tx(w.bar, Piece<T>::PIECES * 512);
+  tma_load_2d(smem_u32(w.res), &maps.res, col0, (int)row0, w.bar);
+}
+// Checkpoint, activation, residual and stores of a warp's 32 x 32 piece, a row
+// per lane in v (bias included). The residual's load is under way (TMA) and
+// replaced by that of next_col (if >= 0). False on a wait that gave up.
+template <class T, bool FULL>
+__device__ __forceinline__ bool finish_piece(const TcArgs& g, const Maps& maps, float (&v)[32], WarpStage& w, int lane, long long row0,
+                                             int col0, int next_col, volatile int* abort_flag) {
+  using P = Piece<T>;
+  const Epilogue& e = g.e;
+  const int rows = (int)(g.m - row0 < 32 ? g.m - row0 : 32);
+  if (lane == 0) tma_store_read();  // the piece before this one has left
+  __syncwarp();
+  if (FULL) {
     if (e.pre) {
-      S::put_row(stg, lane, v);
-      __syncwarp();
-      S::store(stg, lane, (T*)e.pre, g.n, row0, rows, col0, g.n, g.vec_pre);
+      P::put_row(w.out, lane, v);
+      if (g.tma_pre) {
+        fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store(&maps.pre, smem_u32(w.out), col0, (int)row0);
+          tma_store_read();
+        }
+      } else {
+        __syncwarp();
+        P::store_rows(w.out, lane, (T*)e.pre, g.n, row0, rows, col0, g.n);
+      }
       __syncwarp();
     }
     if (e.codes) {
       // the lane's 32 columns are one block of the checkpoint (columns past n count as zeros)
+      const int count = g.n - col0;
       uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) top = max(top, col0 + j < g.n ? __float_as_uint(v[j]) & 0x7FFFFFFFu : 0u);
+      for (int j = 0; j < 32; ++j) top = max(top, j < count ? __float_as_uint(v[j]) & 0x7FFFFFFFu : 0u);
       const uint32_t byte = act8_exponent(top, act8_floor<T>());
       const float inv = act8_inverse(byte);
-      uint32_t w[8];
+      uint32_t c[8];
 #pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        w[p] = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[p] |= (uint32_t)(act8_code(v[4 * p + i], inv, byte == kAct8Nan) & 0xFF) << (8 * i);
-      }
+      for (int p = 0; p < 8; ++p) c[p] = act8_codes4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3], inv, byte == kAct8Nan);
       if (lane < rows) {
         int8_t* dst = e.codes + (row0 + lane) * g.n + col0;
-        if (g.vec_codes && col0 + 32 <= g.n) {
-          reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-          reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        if (g.vec_codes && count >= 32) {
+          reinterpret_cast<uint4*>(dst)[0] = make_uint4(c[0], c[1], c[2], c[3]);
+          reinterpret_cast<uint4*>(dst)[1] = make_uint4(c[4], c[5], c[6], c[7]);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (col0 + j < g.n) dst[j] = (int8_t)(w[j >> 2] >> (8 * (j & 3)));
+            if (j < count) dst[j] = (int8_t)(c[j >> 2] >> (8 * (j & 3)));
         }
         e.exps[(row0 + lane) * act8_blocks(g.n) + (col0 >> 5)] = (uint8_t)byte;
       }
     }
-    act_values(e.act, v);
+    switch (e.act) {
+      case SCMP_ACT_RELU: act_all<SCMP_ACT_RELU>(v); break;
+      case SCMP_ACT_GELU: act_all<SCMP_ACT_GELU>(v); break;
+      case SCMP_ACT_GELU_TANH: act_all<SCMP_ACT_GELU_TANH>(v); break;
+      case SCMP_ACT_SILU: act_all<SCMP_ACT_SILU>(v); break;
+      default: break;
+    }
     if (e.residual) {
-      S::load(stg, lane, (const T*)e.residual, e.ldr, row0, rows, col0, g.n, g.vec_res);
+      if (g.tma_res) {
+        if (!mbar_wait(w.bar, w.phase & 1, abort_flag, 25)) return false;
+        ++w.phase;
+      } else {
+        P::load_rows(w.res, lane, (const T*)e.residual, e.ldr, row0, rows, col0, g.n);
+        __syncwarp();
+      }
+      P::add_row(w.res, lane, v);
       __syncwarp();
-      S::add_row(stg, lane, v);
-      __syncwarp();
+      if (g.tma_res && next_col >= 0 && lane == 0) start_residual<T>(maps, w, row0, next_col);
     }
   }
-  S::put_row(stg, lane, v);
+  P::put_row(w.out, lane, v);
+  if (g.tma_out) {
+    fence_async();
+    __syncwarp();
+    if (lane == 0) tma_store(&maps.out, smem_u32(w.out), col0, (int)row0);
+  } else {
+    __syncwarp();
+    P::store_rows(w.out, lane, (T*)e.out, e.ldo, row0, rows, col0, g.n);
+    __syncwarp();
+  }
+  return true;
+}
+// The bias of `pieces` times 32 columns into scratch (one float per column), and
+// from there the same values into every lane.
+template <class T, int NP>
+__device__ __forceinline__ void bias_rows(const TcArgs& g, float* scratch, int lane, int col0, float (&v)[NP][32]) {
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const int c = col0 + p * 32 + lane;
+    scratch[p * 32 + lane] = c >= g.n ? 0.f : g.e.bias_f32 ? __ldg((const float*)g.e.bias + c) : ldg1((const T*)g.e.bias + c);
+  }
   __syncwarp();
-  S::store(stg, lane, (T*)e.out, e.ldo, row0, rows, col0, g.n, g.vec_out);
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 b = reinterpret_cast<const float4*>(scratch)[p * 8 + q];
+      v[p][4 * q] = b.x;
+      v[p][4 * q + 1] = b.y;
+      v[p][4 * q + 2] = b.z;
+      v[p][4 * q + 3] = b.w;
+    }
   __syncwarp();
 }
 
 template <class T, bool A_MN, bool B_MN, int BN, bool FULL>
 __global__ void __launch_bounds__(TC_THREADS, 1)
-    gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ TcArgs g) {
-  using C = Cfg<BN>;
+    gemm_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ TcArgs g) {
+  using C = Cfg<T, BN>;
   constexpr int NST = C::STAGES;
   extern __shared__ char smem_raw[];
   char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(base);
-  char* tail = base + NST * C::STAGE + C::STG + C::BIAS;
+  char* tail = base + NST * C::STAGE + C::STG;
   const uint32_t bars = smem_u32(tail);
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail + 8 * (2 * NST + 5));
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8 * (2 * NST + 5) + 4);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail + 8 * (2 * NST + 5 + EPI_WARPS));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8 * (2 * NST + 5 + EPI_WARPS) + 4);
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (NST + s); };
   auto accf = [&](int b) { return bars + 8u * (2 * NST + b); };
@@ -290,6 +360,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       mbar_init(acce(b), 2 * EPI_WARPS);
     }
     mbar_init(drain, 1);
+    for (int w = 0; w < EPI_WARPS; ++w) mbar_init(drain + 8 + 8 * w, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -299,8 +370,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   if (warp == 0 && lane == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b) : "memory");
   }
   tc_before();
   __syncthreads();
@@ -308,20 +379,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   tc_after();
   const uint32_t tmem = *tmem_slot;
 
-  const int tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits, total_kb = g.kblocks * g.segments;
+  constexpr bool PROMOTE = FULL || sizeof(T) == 4;
+  const int tiles = g.tiles_m * g.tiles_n, items = g.whole + (tiles - g.whole) * g.splits;
   // Tiles in bands of eight tile rows, column after column within a band, so
   // that the clusters running at a time share A's and B's rows in L2.
+  // Returns the index of the part, or -1 for a whole tile.
   auto place = [&](int item, int& tm, int& tn, int& k0, int& k1) {
-    const int split = item / tiles, t = item - split * tiles;
+    int t = item, part = -1;
+    k0 = 0;
+    k1 = g.kblocks;
+    if (item >= g.whole && g.splits > 1) {
+      part = item - g.whole;
+      const int split = part % g.splits;
+      t = g.whole + part / g.splits;
+      k0 = (int)((long long)g.kblocks * split / g.splits);
+      k1 = (int)((long long)g.kblocks * (split + 1) / g.splits);
+    }
     const int band = t / (8 * g.tiles_n), r = t - band * 8 * g.tiles_n;
     const int h = min(8, g.tiles_m - band * 8);
     tn = r / h;
     tm = band * 8 + r - tn * h;
-    k0 = (int)((long long)total_kb * split / g.splits);
-    k1 = (int)((long long)total_kb * (split + 1) / g.splits);
-    return split;
+    return part;
   };
+  const int chunk = PROMOTE ? g.chunk : g.kblocks;
 
+  if constexpr (PROMOTE) {
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  }
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
@@ -330,8 +414,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         int tm, tn, k0, k1;
         place(item, tm, tn, k0, k1);
         const int i0 = tm * 256 + (int)rank * 128, j0 = tn * BN + (int)rank * (BN / 2);
-        int seg = k0 / g.kblocks, kb = k0 - seg * g.kblocks;
-        for (int k = k0; k < k1; ++k, ++it) {
+        // a chunk of k blocks of every plane pair, chunk after chunk
+        int c0 = k0, seg = 0, kb = k0;
+        for (int left = (k1 - k0) * g.segments; left > 0; --left, ++it) {
           const int s = it % NST;
           if (!mbar_wait(empty(s), ((it / NST) & 1) ^ 1, abort_flag, 20)) {
             ok = false;
@@ -342,20 +427,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           if (rank == 0) expect_tx(full(s), 2 * C::STAGE);
           const int x = kb * KB, pa = g.pa[seg], pb = g.pb[seg];
           if (A_MN) {
-            tma_load(a, &map_a, i0, x, pa, lbar);
-            tma_load(a + 8192, &map_a, i0 + 64, x, pa, lbar);
+            tma_load(a, &maps.a, i0, x, pa, lbar);
+            tma_load(a + 8192, &maps.a, i0 + 64, x, pa, lbar);
           } else {
-            tma_load(a, &map_a, x, i0, pa, lbar);
+            tma_load(a, &maps.a, x, i0, pa, lbar);
           }
           if (B_MN) {
-            tma_load(b, &map_b, j0, x, pb, lbar);
-            if (BN == 256) tma_load(b + 8192, &map_b, j0 + 64, x, pb, lbar);
+            tma_load(b, &maps.b, j0, x, pb, lbar);
+            if (BN == 256) tma_load(b + 8192, &maps.b, j0 + 64, x, pb, lbar);
           } else {
-            tma_load(b, &map_b, x, j0, pb, lbar);
+            tma_load(b, &maps.b, x, j0, pb, lbar);
           }
-          if (++kb == g.kblocks) {
-            kb = 0;
-            ++seg;
+          if (++kb == min(c0 + chunk, k1)) {
+            if (++seg == g.segments) {
+              seg = 0;
+              c0 += chunk;
+            }
+            kb = c0;
           }
         }
       }
@@ -370,28 +458,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const uint64_t ad0 = desc_base(A_MN ? 8192 : 16), bd0 = desc_base(B_MN ? 8192 : 16);
       uint32_t it = 0, n_acc = 0;
       bool ok = true;
-      for (int item = cluster; item < items && ok; item += clusters, ++n_acc) {
+      for (int item = cluster; item < items && ok; item += clusters) {
         int tm, tn, k0, k1;
         place(item, tm, tn, k0, k1);
-        const int buf = n_acc & 1;
-        if (!mbar_wait(acce(buf), ((n_acc >> 1) & 1) ^ 1, abort_flag, 21)) break;
-        tc_after();
-        const uint32_t acc = tmem + buf * ACC_COLS;
-        for (int k = k0; k < k1; ++k, ++it) {
-          const int s = it % NST;
-          if (!mbar_wait(full(s), (it / NST) & 1, abort_flag, 22)) {
+        for (int c0 = k0; c0 < k1 && ok; c0 += chunk, ++n_acc) {
+          const int buf = n_acc & 1, steps = (min(c0 + chunk, k1) - c0) * g.segments;
+          if (!mbar_wait(acce(buf), ((n_acc >> 1) & 1) ^ 1, abort_flag, 21)) {
             ok = false;
             break;
           }
           tc_after();
-          const uint32_t a = sbase + s * C::STAGE, b = a + C::A_BYTES;
-          const uint64_t ad = ad0 | ((a >> 4) & 0x3FFF), bd = bd0 | ((b >> 4) & 0x3FFF);
+          const uint32_t acc = tmem + buf * ACC_COLS;
+          for (int k = 0; k < steps; ++k, ++it) {
+            const int s = it % NST;
+            if (!mbar_wait(full(s), (it / NST) & 1, abort_flag, 22)) {
+              ok = false;
+              break;
+            }
+            tc_after();
+            const uint32_t a = sbase + s * C::STAGE, b = a + C::A_BYTES;
+            const uint64_t ad = ad0 | ((a >> 4) & 0x3FFF), bd = bd0 | ((b >> 4) & 0x3FFF);
 #pragma unroll
-          for (int q = 0; q < KB / 16; ++q)  // 16 k values: 32 bytes along a row, or two 8-k groups
-            mma_f16_pair(acc, ad + q * (A_MN ? 128 : 2), bd + q * (B_MN ? 128 : 2), idesc, (k > k0 || q > 0) ? 1u : 0u);
-          commit_pair(empty(s));
+            for (int q = 0; q < KB / 16; ++q)  // 16 k values: 32 bytes along a row, or two 8-k groups
+              mma_f16_pair(acc, ad + q * (A_MN ? 128 : 2), bd + q * (B_MN ? 128 : 2), idesc, (k > 0 || q > 0) ? 1u : 0u);
+            commit_pair(empty(s));
+          }
+          commit_pair(accf(buf));
         }
-        commit_pair(accf(buf));
       }
       // no MMA is in flight when tensor memory is freed
       asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain) : "memory");
@@ -400,43 +493,104 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     __syncwarp();
   } else if (warp >= 4) {
+    // registers: 384 threads x 168 at launch = 128 x 72 + 256 x 216
+    if constexpr (PROMOTE) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int ew = warp - 4, quad = ew & 3, half = ew >> 2;
-    uint4* stg = reinterpret_cast<uint4*>(base + NST * C::STAGE + ew * 4096);
-    float* bias_s = reinterpret_cast<float*>(base + NST * C::STAGE + C::STG + ew * 128);
+    char* stg = base + NST * C::STAGE + ew * 2 * C::PIECE;
+    WarpStage ws{reinterpret_cast<uint4*>(stg), reinterpret_cast<uint4*>(stg + C::PIECE), drain + 8 + 8 * ew, 0};
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     uint32_t n_acc = 0;
-    for (int item = cluster; item < items; item += clusters, ++n_acc) {
+    bool ok = true;
+    for (int item = cluster; item < items && ok; item += clusters) {
       int tm, tn, k0, k1;
-      const int split = place(item, tm, tn, k0, k1);
-      const int buf = n_acc & 1;
-      if (!mbar_wait(accf(buf), (n_acc >> 1) & 1, abort_flag, 24)) break;
-      tc_after();
+      const int part = place(item, tm, tn, k0, k1);
       const long long row0 = (long long)tm * 256 + rank * 128 + quad * 32;
-      const int rows = (int)(g.m - row0 < 32 ? (g.m > row0 ? g.m - row0 : 0) : 32);
-#pragma unroll 1
-      for (int c = 0; c < BN / 64; ++c) {
-        const int tc = half * (BN / 2) + c * 32, col0 = tn * BN + tc;
-        uint32_t r[32];
-        tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + buf * ACC_COLS + tc, r);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (c == BN / 64 - 1) {  // the accumulator is read: the next tile's MMAs may overwrite it
-          tc_before();
+      const int cols0 = tn * BN + half * (BN / 2);
+      const bool live = row0 < g.m && cols0 < g.n;
+      if (FULL && g.e.residual && g.tma_res && live && part < 0 && lane == 0) start_residual<T>(maps, ws, row0, cols0);
+      // piece p of the tile, its sums in v
+      auto emit = [&](int p, float (&v)[32]) {
+        const int col0 = cols0 + p * 32;
+        if (row0 >= g.m || col0 >= g.n) return;
+        if (part >= 0) {  // in the order in which join_kernel's lanes read it
+          float4* dst = reinterpret_cast<float4*>(g.partial) +
+                        ((((size_t)part * 2 + rank) * 4 + quad) * (BN / 32) + half * C::NP + p) * 256 + lane;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) dst[q * 32] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        } else {
+          ok = finish_piece<T, FULL>(g, maps, v, ws, lane, row0, col0, p + 1 < C::NP && col0 + 32 < g.n ? col0 + 32 : -1, abort_flag);
+        }
+      };
+      if constexpr (PROMOTE) {
+        float sum[C::NP][32];
+        if (FULL && g.e.bias && part < 0) {
+          if (lane == 0) tma_store_read();
+          __syncwarp();
+          bias_rows<T>(g, reinterpret_cast<float*>(ws.out), lane, cols0, sum);
+        } else {
+#pragma unroll
+          for (int p = 0; p < C::NP; ++p)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[p][j] = 0.f;
+        }
+        for (int c0 = k0; c0 < k1; c0 += chunk, ++n_acc) {
+          const int buf = n_acc & 1;
+          if (!mbar_wait(accf(buf), (n_acc >> 1) & 1, abort_flag, 24)) {
+            ok = false;
+            break;
+          }
+          tc_after();
+          const uint32_t src = tmem + lanes + buf * ACC_COLS + half * (BN / 2);
+          // the next 16 columns are on their way while these are added
+          uint32_t r[2][16];
+          tmem_ld16(src, r[0]);
+#pragma unroll
+          for (int q = 0; q < 2 * C::NP; ++q) {
+            tmem_wait();
+            if (q + 1 < 2 * C::NP) tmem_ld16(src + (q + 1) * 16, r[(q + 1) & 1]);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[q >> 1][(q & 1) * 16 + j] += __uint_as_float(r[q & 1][j]);
+          }
+          tc_before();  // the accumulator is read: the MMAs may overwrite it
           __syncwarp();
           if (lane == 0) arrive_cluster(leader_addr(acce(buf)));
         }
-        if (rows == 0 || col0 >= g.n) continue;
-        float v[32];
+        // one copy of the epilogue's code, which would not fit the instruction cache four times
+#pragma unroll 1
+        for (int p = 0; p < C::NP && ok; ++p) {
+          float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        if (g.partial) {
-          Stage<float>::put_row(stg, lane, v);
-          __syncwarp();
-          Stage<float>::store(stg, lane, g.partial + (size_t)split * g.m * g.n, g.n, row0, rows, col0, g.n, g.n % 4 == 0);
-          __syncwarp();
-        } else {
-          finish_piece<T, FULL>(g, v, stg, bias_s, lane, row0, rows, col0);
+          for (int j = 0; j < 32; ++j) {
+            v[j] = sum[0][j];
+#pragma unroll
+            for (int i = 1; i < C::NP; ++i) v[j] = p == i ? sum[i][j] : v[j];
+          }
+          emit(p, v);
         }
+      } else {
+        const int buf = n_acc & 1;
+        if (!mbar_wait(accf(buf), (n_acc >> 1) & 1, abort_flag, 24)) break;
+        tc_after();
+#pragma unroll 1
+        for (int p = 0; p < C::NP; ++p) {
+          uint32_t r[32];
+          tmem_ld32(tmem + lanes + buf * ACC_COLS + half * (BN / 2) + p * 32, r);
+          tmem_wait();
+          if (p == C::NP - 1) {
+            tc_before();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(leader_addr(acce(buf)));
+          }
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          emit(p, v);
+        }
+        ++n_acc;
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
   if (*abort_flag) {
     // a wait gave up: let the copies in flight land before shared memory goes
@@ -450,46 +604,49 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Adds the partial products in order and runs the epilogue: a lane per column
-// (32 columns are one block of an 8-bit checkpoint), JOIN_ROWS rows per warp at
-// a time so that their loads overlap.
-constexpr int JOIN_ROWS = 4;
+// Adds the partial tiles in order and runs the epilogue: a warp per 32 x 32 piece.
 template <class T, bool FULL>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs g) {
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Maps maps, const __grid_constant__ TcArgs g, int bn) {
+  __shared__ __align__(1024) uint4 stg[4][2][Piece<T>::PIECES * 32];
+  __shared__ uint64_t bars[4];
+  __shared__ int abort_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row0 = ((long long)blockIdx.y * 8 + warp) * JOIN_ROWS;
-  const int col = blockIdx.x * 32 + lane;
-  const bool live = col < g.n;
-  const Epilogue& e = g.e;
-  float v[JOIN_ROWS];
+  const int t = g.whole + blockIdx.y, band = t / (8 * g.tiles_n), r0 = t - band * 8 * g.tiles_n;
+  const int h = min(8, g.tiles_m - band * 8), tn = r0 / h, tm = band * 8 + r0 - tn * h;
+  const int piece = blockIdx.x * 4 + warp, strip = piece / (bn / 32), cp = piece - strip * (bn / 32);
+  const long long row0 = (long long)tm * 256 + strip * 32;
+  const int col0 = tn * bn + cp * 32;
+  WarpStage ws{stg[warp][0], stg[warp][1], smem_u32(&bars[warp]), 0};
+  if (lane == 0) {
+    mbar_init(ws.bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0) abort_s = 0;
+  __syncthreads();
+  if (row0 >= g.m || col0 >= g.n) return;  // whole warps
+  if (FULL && g.e.residual && g.tma_res && lane == 0) start_residual<T>(maps, ws, row0, col0);
+  float v[1][32];
+  if (FULL && g.e.bias) {
+    bias_rows<T>(g, reinterpret_cast<float*>(ws.out), lane, col0, v);
+  } else {
 #pragma unroll
-  for (int r = 0; r < JOIN_ROWS; ++r) v[r] = 0.f;
-#pragma unroll 4
+    for (int j = 0; j < 32; ++j) v[0][j] = 0.f;
+  }
+  const size_t part_size = (size_t)64 * bn;  // float4s of a partial tile
+  const float4* p = reinterpret_cast<const float4*>(g.partial) + (size_t)blockIdx.y * g.splits * part_size + (size_t)piece * 256 + lane;
+#pragma unroll 2
   for (int s = 0; s < g.splits; ++s) {
-    const float* p = g.partial + ((size_t)s * g.m + row0) * g.n + col;
 #pragma unroll
-    for (int r = 0; r < JOIN_ROWS; ++r)
-      if (live && row0 + r < g.m) v[r] += __ldg(p + (size_t)r * g.n);
-  }
-  const float bias = FULL && e.bias && live ? (e.bias_f32 ? __ldg((const float*)e.bias + col) : ldg1((const T*)e.bias + col)) : 0.f;
-#pragma unroll
-  for (int r = 0; r < JOIN_ROWS; ++r) {
-    const long long row = row0 + r;
-    if (row >= g.m) break;  // whole warps
-    float y = v[r];
-    if (FULL) {
-      y += bias;
-      if (e.pre && live) ((T*)e.pre)[row * g.n + col] = Elem<T>::from_f(y);
-      if (e.codes) {
-        const uint32_t byte = act8_exponent(__reduce_max_sync(0xffffffffu, live ? __float_as_uint(y) & 0x7FFFFFFFu : 0u), act8_floor<T>());
-        if (live) e.codes[row * g.n + col] = (int8_t)act8_code(y, act8_inverse(byte), byte == kAct8Nan);
-        if (lane == 0) e.exps[row * act8_blocks(g.n) + blockIdx.x] = (uint8_t)byte;
-      }
-      y = act_value(e.act, y);
-      if (e.residual && live) y += ldg1((const T*)e.residual + row * e.ldr + col);
+    for (int q = 0; q < 8; ++q) {
+      const float4 f = __ldg(p + s * part_size + q * 32);
+      v[0][4 * q] += f.x;
+      v[0][4 * q + 1] += f.y;
+      v[0][4 * q + 2] += f.z;
+      v[0][4 * q + 3] += f.w;
     }
-    if (live) ((T*)e.out)[row * e.ldo + col] = Elem<T>::from_f(y);
   }
+  finish_piece<T, FULL>(g, maps, v[0], ws, lane, row0, col0, -1, &abort_s);
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -529,49 +686,67 @@ static bool make_map(CUtensorMap* map, const Operand& o, bool f16, int tile_rows
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tile width and number of k splits of a product.
+// A tensor of the epilogue in 32 x 32 boxes.
+static bool make_piece_map(CUtensorMap* map, const void* p, long long rows, int cols, long long ld, int dtype) {
+  const size_t es = dtype_size(dtype);
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * es};
+  const cuuint32_t box[2] = {32, 32}, one[2] = {1, 1};
+  const CUtensorMapDataType t = dtype == SCMP_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : dtype == SCMP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode_tiled()(map, t, 2, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        es == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Tile width, the tiles that run whole, and the k splits of the others.
 struct Schedule {
-  int bn, splits;
+  int bn, tiles_m, tiles_n, whole, splits;
 };
-// Least estimated time, in SM clocks: waves of tiles over 74 SM pairs; a k block
-// takes 560 clocks for 256 columns and 440 for 128 (32 and 24 KB per SM, at the
-// 55 to 58 bytes per clock that L2 delivers to an SM: measured 566 and 444 on
-// 4096 x 4096 x 11008); 2500 per tile that nothing hides; for a split product
-// the partial tiles' way through L2 and a second launch.
-static Schedule schedule_for(long long m, int n, long long kblocks) {
-  Schedule best{256, 1};
+constexpr int PAIRS = 74;  // SM pairs
+// Least estimated time, in SM clocks. A k block takes 560 clocks for 256 columns
+// and 440 for 128 (32 and 24 KB per SM, at the 55 to 58 bytes per clock that L2
+// delivers to an SM: measured 566 and 444 on 4096 x 4096 x 11008), a tile 2500
+// more that nothing hides. Tiles beyond whole waves may be split: then their parts
+// fill waves of their own, and the partial tiles' way through L2 and a second
+// launch come on top.
+static Schedule schedule_for(long long m, int n, int kblocks, int segments) {
+  Schedule best{};
   double least = 1e300;
-  const long long pairs = 74;
   for (int bn : {256, 128}) {
-    const long long tiles = ((m + 255) / 256) * ((n + bn - 1) / bn);
-    for (int s = 1; s <= 16 && (s == 1 || kblocks / s >= 4); ++s) {
-      const long long waves = (tiles * s + pairs - 1) / pairs;
-      double t = waves * ((kblocks + s - 1) / s * (bn == 256 ? 560.0 : 440.0) + 2500.0);
-      if (s > 1) t += 5000.0 + (double)m * n * (s + 1) * 4 / 2500.0;
+    const long long tm = (m + 255) / 256, tn = (n + bn - 1) / bn, tiles = tm * tn;
+    const double block = (bn == 256 ? 560.0 : 440.0) * segments, tile = kblocks * block + 2500.0;
+    const long long whole = tiles / PAIRS * PAIRS, rest = tiles - whole;
+    for (int s = 1; s <= 16 && (s == 1 || (kblocks / s >= 2 && rest)); ++s) {
+      double t = whole / PAIRS * tile;
+      if (s == 1)
+        t += rest ? tile : 0.0;
+      else
+        t += (rest * s + PAIRS - 1) / PAIRS * (((kblocks + s - 1) / s) * block + 2500.0) + 5000.0 + (double)rest * (s + 1) * 256 * bn * 4 / 2500.0;
       if (t < least) {
         least = t;
-        best = {bn, s};
+        best = {bn, (int)tm, (int)tn, (int)(s == 1 ? tiles : whole), s};
       }
     }
   }
   return best;
 }
-static int plane_pairs(int planes_a, int planes_b) { return planes_a == 1 ? planes_b : planes_b == 1 ? planes_a : 6; }
-static size_t partial_bytes(long long m, int n, long long kblocks) {
-  const Schedule s = schedule_for(m, n, kblocks);
-  return s.splits > 1 ? (size_t)s.splits * m * n * sizeof(float) : 0;
+static size_t partial_bytes(long long m, int n, int kblocks, int segments) {
+  const Schedule s = schedule_for(m, n, kblocks, segments);
+  return (size_t)(s.tiles_m * s.tiles_n - s.whole) * s.splits * 256 * s.bn * sizeof(float);
 }
+static int plane_pairs(int planes_a, int planes_b) { return planes_a == 1 ? planes_b : planes_b == 1 ? planes_a : 6; }
 
 template <class T, bool A_MN, bool B_MN, int BN, bool FULL>
-static cudaError_t launch_tc_t(const CUtensorMap& ma, const CUtensorMap& mb, const TcArgs& g, cudaStream_t st) {
+static cudaError_t launch_tc_t(const Maps& maps, const TcArgs& g, cudaStream_t st) {
   auto kern = gemm_tc_kernel<T, A_MN, B_MN, BN, FULL>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN>::SMEM);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (Cfg<T, BN>::SMEM));
   if (e != cudaSuccess) return e;
-  const long long items = (long long)g.tiles_m * g.tiles_n * g.splits;
+  const int rest = g.tiles_m * g.tiles_n - g.whole;
+  const long long items = g.whole + (long long)rest * g.splits;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * (items < 74 ? items : 74)), 1, 1);
+  cfg.gridDim = dim3((unsigned)(2 * (items < PAIRS ? items : PAIRS)), 1, 1);
   cfg.blockDim = dim3(TC_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = Cfg<BN>::SMEM;
+  cfg.dynamicSmemBytes = (Cfg<T, BN>::SMEM);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -580,10 +755,10 @@ static cudaError_t launch_tc_t(const CUtensorMap& ma, const CUtensorMap& mb, con
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, ma, mb, g);
+  e = cudaLaunchKernelEx(&cfg, kern, maps, g);
   count_launch();
-  if (e == cudaSuccess && g.splits > 1) {
-    join_kernel<T, FULL><<<dim3(cdiv(g.n, 32), (unsigned)((g.m + 8LL * JOIN_ROWS - 1) / (8 * JOIN_ROWS))), 256, 0, st>>>(g);
+  if (e == cudaSuccess && rest > 0) {
+    join_kernel<T, FULL><<<dim3(BN / 32 * 8 / 4, rest), 128, 0, st>>>(maps, g, BN);
     count_launch();
     e = cudaGetLastError();
   }
@@ -605,27 +780,33 @@ static cudaError_t launch_tc(const Operand& a, const Operand& b, long long m, in
     g.pa[s] = b.planes == 1 ? g.segments - 1 - s : a.planes == 1 ? 0 : six_a[s];
     g.pb[s] = a.planes == 1 ? g.segments - 1 - s : b.planes == 1 ? 0 : six_b[s];
   }
-  const Schedule sc = schedule_for(m, n, (long long)g.kblocks * g.segments);
-  g.tiles_m = (int)((m + 255) / 256);
-  g.tiles_n = cdiv(n, sc.bn);
+  g.chunk = dtype == SCMP_F32 ? 4 : 16;
+  const Schedule sc = schedule_for(m, n, g.kblocks, g.segments);
+  g.tiles_m = sc.tiles_m;
+  g.tiles_n = sc.tiles_n;
+  g.whole = sc.whole;
   g.splits = sc.splits;
   g.f16 = dtype == SCMP_F16;
-  g.partial = sc.splits > 1 ? partial : nullptr;
+  g.partial = partial;
   g.e = e;
   const size_t es = dtype_size(dtype);
-  g.vec_out = rows_aligned16(e.out, e.ldo, es);
-  g.vec_res = rows_aligned16(e.residual, e.ldr, es);
-  g.vec_pre = rows_aligned16(e.pre, n, es);
+  g.tma_out = rows_aligned16(e.out, e.ldo, es);
+  g.tma_res = e.residual && rows_aligned16(e.residual, e.ldr, es);
+  g.tma_pre = e.pre && rows_aligned16(e.pre, n, es);
   g.vec_codes = aligned16(e.codes) && n % 16 == 0;
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, a, g.f16, 128) || !make_map(&mb, b, g.f16, sc.bn / 2)) return cudaErrorInvalidValue;
+  Maps maps;
+  if (!make_map(&maps.a, a, g.f16, 128) || !make_map(&maps.b, b, g.f16, sc.bn / 2) ||
+      (g.tma_out && !make_piece_map(&maps.out, e.out, m, n, e.ldo, dtype)) ||
+      (g.tma_res && !make_piece_map(&maps.res, e.residual, m, n, e.ldr, dtype)) ||
+      (g.tma_pre && !make_piece_map(&maps.pre, e.pre, m, n, n, dtype)))
+    return cudaErrorInvalidValue;
   return with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     if (!a.mn && !b.mn)
-      return sc.bn == 256 ? launch_tc_t<T, false, false, 256, true>(ma, mb, g, st) : launch_tc_t<T, false, false, 128, true>(ma, mb, g, st);
+      return sc.bn == 256 ? launch_tc_t<T, false, false, 256, true>(maps, g, st) : launch_tc_t<T, false, false, 128, true>(maps, g, st);
     if (!a.mn)
-      return sc.bn == 256 ? launch_tc_t<T, false, true, 256, false>(ma, mb, g, st) : launch_tc_t<T, false, true, 128, false>(ma, mb, g, st);
-    return sc.bn == 256 ? launch_tc_t<T, true, true, 256, false>(ma, mb, g, st) : launch_tc_t<T, true, true, 128, false>(ma, mb, g, st);
+      return sc.bn == 256 ? launch_tc_t<T, false, true, 256, false>(maps, g, st) : launch_tc_t<T, false, true, 128, false>(maps, g, st);
+    return sc.bn == 256 ? launch_tc_t<T, true, true, 256, false>(maps, g, st) : launch_tc_t<T, true, true, 128, false>(maps, g, st);
   });
 }
 

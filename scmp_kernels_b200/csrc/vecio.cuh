@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace scmp {
@@ -73,18 +75,59 @@ __device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f(e[i]);
 }
+// Two values as a 32-bit word of the 16-bit type, one conversion.
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
 template <class T>
 __device__ __forceinline__ void stg8(T* p, const float (&v)[8]) {
   Raw8<T> r;
-  T* e = reinterpret_cast<T*>(&r);
+  if constexpr (sizeof(T) == 2) {
+    r.q[0] = make_uint4(pack2(v[0], v[1], p), pack2(v[2], v[3], p), pack2(v[4], v[5], p), pack2(v[6], v[7], p));
+  } else {
+    T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_f(v[i]);
+    for (int i = 0; i < 8; ++i) e[i] = v[i];
+  }
   uint4* d = reinterpret_cast<uint4*>(p);
 #pragma unroll
   for (int i = 0; i < (int)(sizeof(T) * 8 / 16); ++i) d[i] = r.q[i];
 }
 
+// Four consecutive values as they lie in memory (8 or 16 bytes, aligned to that).
+template <class T>
+struct Raw4 {
+  using U = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+  U q;
+};
+template <class T>
+__device__ __forceinline__ Raw4<T> ldg4(const T* p) {
+  return {__ldg(reinterpret_cast<const typename Raw4<T>::U*>(p))};
+}
+template <class T>
+__device__ __forceinline__ void unpack4(const Raw4<T>& r, float (&v)[4]) {
+  const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = Elem<T>::to_f(e[i]);
+}
+template <class T>
+__device__ __forceinline__ void stg4(T* p, const float (&v)[4]) {
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v[0], v[1], p), pack2(v[2], v[3], p));
+  else
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Rows at a pitch of ld elements can be accessed four elements at a time.
+inline bool rows_aligned4(const void* p, long long ld, size_t esize) {
+  return reinterpret_cast<uintptr_t>(p) % (4 * esize) == 0 && ld % 4 == 0;
+}
 // Rows of `cols` elements at a pitch of ld elements can be read 16 bytes at a time.
 inline bool rows_aligned16(const void* p, long long ld, size_t esize) {
   return aligned16(p) && (size_t)ld * esize % 16 == 0;
