@@ -332,7 +332,7 @@ int scmp_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, i
 int scmp_layer_norm_forward(const void* x, int dtype, long long rows, int cols, long long ldx,
                             const void* weight, const void* bias, int wdtype, float eps, void* y,
                             float* mean, float* rstd, int8_t* codes, uint8_t* exps, void* stream);
-int scmp_layer_norm_backward_workspace_size(long long rows, int cols, size_t* bytes);
+int scmp_layer_norm_backward_workspace_size(int dtype, long long rows, int cols, size_t* bytes);
 int scmp_layer_norm_backward(const void* dy, long long lddy, const void* x, long long ldx,
                              const int8_t* codes, const uint8_t* exps, int dtype, long long rows,
                              int cols, const float* mean, const float* rstd, const void* weight,

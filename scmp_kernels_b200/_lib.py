@@ -103,7 +103,7 @@ SIGNATURES = {
     "scmp_act8_unpack": (c_int, [c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p]),
     "scmp_layer_norm_forward": (c_int, [c_void_p, c_int, c_longlong, c_int, c_longlong, c_void_p, c_void_p, c_int,
                                         c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "scmp_layer_norm_backward_workspace_size": (c_int, [c_longlong, c_int, ctypes.POINTER(c_size_t)]),
+    "scmp_layer_norm_backward_workspace_size": (c_int, [c_int, c_longlong, c_int, ctypes.POINTER(c_size_t)]),
     "scmp_layer_norm_backward": (c_int, [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p, c_int,
                                          c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_size_t, c_void_p]),

@@ -4,80 +4,140 @@
 
 namespace scmp {
 
-// Four threads hold a block of 32 values, eight each.
+// VEC: four threads hold a block of 32 values, eight each, two blocks in flight.
+// Else a warp holds a block, a lane per value, four blocks in flight.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x, long long rows, int cols, long long ld,
-                                                        int8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
-  const int nb = act8_blocks(cols);
-  const int quarter = threadIdx.x & 3;
-  const long long stride = (long long)gridDim.x * (blockDim.x >> 2);
+                                                        int8_t* __restrict__ codes, uint8_t* __restrict__ exps, FastDiv by) {
+  const int nb = act8_blocks(cols), lane = threadIdx.x & 31;
   const long long total = rows * nb;
-  // whole warps stay in the loop for the shuffles
-  for (long long blk0 = (long long)blockIdx.x * (blockDim.x >> 2) + ((threadIdx.x >> 5) << 3); blk0 < total; blk0 += stride) {
-    const long long blk = blk0 + ((threadIdx.x & 31) >> 2);
-    const bool live = blk < total;
-    const long long row = live ? blk / nb : 0;
-    const int b = (int)(live ? blk - row * nb : 0);
-    const int c0 = b * kAct8Block + quarter * 8;
-    const T* src = x + row * ld + c0;
-    float v[8];
-    if (VEC) {
-      if (live && c0 < cols) {
-        unpack8(ldg8(src), v);
-      } else {
+  const bool small = total < 1LL << 31;
+  if constexpr (VEC) {
+    constexpr int U = 2;
+    const int quarter = threadIdx.x & 3;
+    const long long stride = (long long)gridDim.x * 64;
+    // whole warps stay in the loop for the shuffles
+    for (long long b0 = (long long)blockIdx.x * 64 + ((threadIdx.x >> 5) << 3); b0 < total; b0 += U * stride) {
+      Raw8<T> raw[U];
+      long long row[U];
+      int c[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      for (int u = 0; u < U; ++u) {
+        const long long blk = b0 + u * stride + (lane >> 2);
+        row[u] = 0;
+        c[u] = cols;
+        if (blk < total) {
+          row_and_piece(blk, by, small, row[u], c[u]);
+          c[u] = c[u] * kAct8Block + quarter * 8;
+        }
+        if (c[u] < cols) raw[u] = ldg8(x + row[u] * ld + c[u]);
       }
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = live && c0 + i < cols ? Elem<T>::to_f(src[i]) : 0.f;
+      for (int u = 0; u < U; ++u) {
+        float v[8];
+        unpack8(raw[u], v);
+        uint32_t top = 0;
+        if (c[u] < cols) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t byte = act8_exponent(top, act8_floor<T>());
+        const float inv = act8_inverse(byte);
+        const bool nan = byte == kAct8Nan;
+        if (c[u] >= cols) continue;
+        *reinterpret_cast<uint2*>(codes + row[u] * cols + c[u]) =
+            make_uint2(act8_codes4(v[0], v[1], v[2], v[3], inv, nan), act8_codes4(v[4], v[5], v[6], v[7], inv, nan));
+        if (quarter == 0) exps[row[u] * nb + (c[u] >> 5)] = (uint8_t)byte;
+      }
     }
-    uint32_t top = 0;
+  } else {
+    constexpr int U = 4;
+    const long long stride = (long long)gridDim.x * 8;
+    for (long long b0 = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); b0 < total; b0 += U * stride) {
+      float v[U];
+      long long at[U];
+      bool live[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t byte = act8_exponent(top, act8_floor<T>());
-    const float inv = act8_inverse(byte);
-    const bool nan = byte == kAct8Nan;
-    const uint32_t w[2] = {act8_codes4(v[0], v[1], v[2], v[3], inv, nan), act8_codes4(v[4], v[5], v[6], v[7], inv, nan)};
-    if (!live) continue;
-    int8_t* dst = codes + row * cols + c0;
-    if (VEC) {
-      if (c0 < cols) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-    } else {
+      for (int u = 0; u < U; ++u) {
+        const long long blk = b0 + u * stride;
+        long long row = 0;
+        int c = 0;
+        if (blk < total) row_and_piece(blk, by, small, row, c);
+        c = c * kAct8Block + lane;
+        live[u] = blk < total && c < cols;
+        at[u] = row * cols + c;
+        v[u] = live[u] ? ldg1(x + row * ld + c) : 0.f;
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c0 + i < cols) dst[i] = (int8_t)(w[i >> 2] >> (8 * (i & 3)));
+      for (int u = 0; u < U; ++u) {
+        const uint32_t byte = act8_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(v[u]) & 0x7FFFFFFFu), act8_floor<T>());
+        if (live[u]) codes[at[u]] = (int8_t)act8_code(v[u], act8_inverse(byte), byte == kAct8Nan);
+        if (lane == 0 && b0 + u * stride < total) exps[b0 + u * stride] = (uint8_t)byte;
+      }
     }
-    if (quarter == 0) exps[blk] = (uint8_t)byte;
   }
 }
 
+// A thread writes 16 bytes (four or eight values), neighbouring threads
+// neighbouring ones, four such pieces in flight.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) act8_unpack_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
-                                                          long long rows, int cols, long long ldo,
-                                                          T* __restrict__ out) {
+                                                          long long rows, int cols, long long ldo, T* __restrict__ out, FastDiv by) {
   const int nb = act8_blocks(cols);
-  const long long total = rows * nb * 4;
-  const long long stride = (long long)gridDim.x * blockDim.x;
-  for (long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x; t < total; t += stride) {
-    const long long blk = t >> 2, row = blk / nb;
-    const int b = (int)(blk - row * nb), c0 = b * kAct8Block + (int)(t & 3) * 8;
-    if (c0 >= cols) continue;
-    const float s = act8_scale(__ldg(exps + blk));
-    const int8_t* src = codes + row * cols + c0;
-    T* dst = out + row * ldo + c0;
-    if (VEC) {
-      const uint2 q = __ldg(reinterpret_cast<const uint2*>(src));
-      float v[8];
+  if constexpr (VEC) {
+    constexpr int PER = 16 / sizeof(T), U = 4;
+    const int per_row = cols / PER;
+    const long long total = rows * per_row, stride = (long long)gridDim.x * 256;
+    for (long long t0 = (long long)blockIdx.x * 256 + threadIdx.x; t0 < total; t0 += U * stride) {
+      uint32_t q[U][PER / 4];
+      uint32_t ex[U];
+      long long at[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act8_value(i < 4 ? q.x : q.y, i & 3, s);
-      stg8(dst, v);
-    } else {
+      for (int u = 0; u < U; ++u) {
+        const long long t = t0 + u * stride;
+        at[u] = -1;
+        if (t >= total) continue;
+        long long row;
+        int c;
+        row_and_piece(t, by, total < 1LL << 31, row, c);
+        c *= PER;
+        at[u] = row * ldo + c;
+        ex[u] = __ldg(exps + row * nb + (c >> 5));
+        const int8_t* src = codes + row * cols + c;
+        if constexpr (PER == 8) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+          q[u][0] = w.x;
+          q[u][1] = w.y;
+        } else {
+          q[u][0] = __ldg(reinterpret_cast<const unsigned int*>(src));
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c0 + i < cols) dst[i] = Elem<T>::from_f(fmul((float)src[i], s));
+      for (int u = 0; u < U; ++u) {
+        if (at[u] < 0) continue;
+        const float s = act8_scale(ex[u]);
+        float v[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = act8_value(q[u][i >> 2], i & 3, s);
+        if constexpr (PER == 8)
+          stg8(out + at[u], v);
+        else
+          stg4(out + at[u], v);
+      }
+    }
+  } else {
+    // a warp per block of 32, a lane per value
+    const int lane = threadIdx.x & 31;
+    const long long total = rows * nb, stride = (long long)gridDim.x * 8;
+#pragma unroll 4
+    for (long long blk = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); blk < total; blk += stride) {
+      long long row;
+      int c;
+      row_and_piece(blk, by, total < 1LL << 31, row, c);
+      c = c * 32 + lane;
+      if (c < cols) out[row * ldo + c] = Elem<T>::from_f(fmul((float)__ldg(codes + row * cols + c), act8_scale(__ldg(exps + blk))));
     }
   }
 }
@@ -90,13 +150,13 @@ static int elementwise_grid(long long items, int per_block) {
 cudaError_t launch_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, int cols, void* out,
                                long long ldo, int dtype, cudaStream_t st) {
   const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && rows_aligned16(out, ldo, dtype_size(dtype));
-  const int grid = elementwise_grid(rows * act8_blocks(cols) * 4, 256);
+  const int grid = elementwise_grid(rows * act8_blocks(cols) * 4, vec ? 256 : 32);
   with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     if (vec)
-      act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, exps, rows, cols, ldo, (T*)out);
+      act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, exps, rows, cols, ldo, (T*)out, FastDiv(cols / (16 / sizeof(T))));
     else
-      act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, exps, rows, cols, ldo, (T*)out);
+      act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, exps, rows, cols, ldo, (T*)out, FastDiv(act8_blocks(cols)));
   });
   count_launch();
   return cudaGetLastError();
@@ -116,13 +176,13 @@ int scmp_act8_pack(const void* x, int dtype, long long rows, int cols, long long
   if (!x || !codes || !exps) return fail(SCMP_ERR_INVALID_ARG, "act8_pack: null pointer");
   const cudaStream_t st = (cudaStream_t)stream;
   const bool vec = cols % 8 == 0 && rows_aligned16(x, ld, dtype_size(dtype)) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
-  const int grid = elementwise_grid(rows * act8_blocks(cols) * 4, 256);
+  const int grid = elementwise_grid(rows * act8_blocks(cols) * 4, vec ? 256 : 32);
   with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     if (vec)
-      act8_pack_kernel<T, true><<<grid, 256, 0, st>>>((const T*)x, rows, cols, ld, codes, exps);
+      act8_pack_kernel<T, true><<<grid, 256, 0, st>>>((const T*)x, rows, cols, ld, codes, exps, FastDiv(act8_blocks(cols)));
     else
-      act8_pack_kernel<T, false><<<grid, 256, 0, st>>>((const T*)x, rows, cols, ld, codes, exps);
+      act8_pack_kernel<T, false><<<grid, 256, 0, st>>>((const T*)x, rows, cols, ld, codes, exps, FastDiv(act8_blocks(cols)));
   });
   count_launch();
   SCMP_CUDA(cudaGetLastError(), "act8_pack");

@@ -59,10 +59,17 @@ __device__ __forceinline__ uint32_t act8_codes4(float a, float b, float c, float
 // The value of byte i of a word of codes: the byte (offset by 128) becomes the
 // low mantissa bits of 2^23, which is then subtracted. Conversions from
 // integers would share the pipe of exp2 and reciprocal.
-__device__ __forceinline__ float act8_value(uint32_t codes, int i, float scale) {
+__device__ __forceinline__ float act8_whole(uint32_t codes, int i) {
   const uint32_t u = __byte_perm(codes ^ 0x80808080u, 0x4B000000u, 0x7650 | i);
-  return fmul(fsub(__uint_as_float(u), 8388736.f), scale);
+  return fsub(__uint_as_float(u), 8388736.f);
 }
+// Codes 2i and 2i + 1 of a word, as whole numbers.
+__device__ __forceinline__ F2 act8_pair(uint32_t codes, int i) {
+  const uint32_t u = codes ^ 0x80808080u;
+  return add2(f2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 | (2 * i))),
+                 __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 | (2 * i + 1)))), f2(-8388736.f));
+}
+__device__ __forceinline__ float act8_value(uint32_t codes, int i, float scale) { return fmul(act8_whole(codes, i), scale); }
 
 // The values of a checkpoint as rows of type dtype at a pitch of ldo (act8.cu).
 cudaError_t launch_act8_unpack(const int8_t* codes, const uint8_t* exps, long long rows, int cols, void* out,

@@ -227,7 +227,7 @@ py::tuple layer_norm_backward(const Tensor& dy, const Tensor& x, const Opt& exps
   if (w.defined()) dw = make({cols}, wtype, dy);
   if (with_bias) db = make({cols}, wtype, dy);
   size_t bytes = 0;
-  if (w.defined() || with_bias) check(scmp_layer_norm_backward_workspace_size(g.rows, narrow(who, cols), &bytes), who);
+  if (w.defined() || with_bias) check(scmp_layer_norm_backward_workspace_size(dt, g.rows, narrow(who, cols), &bytes), who);
   Workspace ws = workspace(bytes, dy);
   check(scmp_layer_norm_backward(g.p(), g.pitch, r.p(), r.pitch, exps ? (const int8_t*)x.const_data_ptr() : nullptr,
                                  cptr<uint8_t>(exps), dt, g.rows, narrow(who, cols), (const float*)mu.const_data_ptr(),

@@ -19,7 +19,9 @@
 namespace scmp {
 namespace ln {
 
-constexpr int kMaxFused = 16384;  // columns held in registers (512 threads x 4 x 8)
+// Columns held in registers: 512 threads x 4 x 8 in the forward pass, half of that
+// beside the sums of the backward pass.
+constexpr int kMaxForward = 16384, kMaxBackward = 8192;
 
 struct Args {
   long long rows, ldx, ldy, ldo;  // row pitches of x, dy and the result (y or dx), in elements
@@ -49,79 +51,141 @@ __device__ __forceinline__ int col_of(int t, int i, int j) {
   return VEC ? (t + TPR * i) * 8 + j : (i * 8 + j) * TPR + t;
 }
 
+// A chunk of a row as it lies in memory, so that the next row's loads can be
+// under way while a row is worked on.
+template <class T, bool SRC8, bool VEC>
+struct Raw;
+template <class T>
+struct Raw<T, false, true> {
+  Raw8<T> q;
+};
+template <class T>
+struct Raw<T, true, true> {
+  uint2 q;
+  uint32_t ex;
+};
+template <class T>
+struct Raw<T, false, false> {
+  T v[8];
+};
+template <class T>
+struct Raw<T, true, false> {
+  float v[8];
+};
+// row: of x (or of its checkpoint's codes and exps).
 template <class T, bool VEC, int TPR>
-__device__ __forceinline__ void load_chunk(const T* __restrict__ row, int cols, int t, int i, float (&v)[8]) {
-  if (VEC) {
+__device__ __forceinline__ void fetch(Raw<T, false, VEC>& r, const T* __restrict__ row, int cols, int t, int i) {
+  if constexpr (VEC) {
+    const int c = (t + TPR * i) * 8;
+    if (c < cols) r.q = ldg8(row + c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = col_of<false, TPR>(t, i, j);
+      if (c < cols) r.v[j] = ldg_raw(row + c);
+    }
+  }
+}
+template <class T, bool VEC, int TPR>
+__device__ __forceinline__ void fetch8(Raw<T, true, VEC>& r, const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps, int cols,
+                                       int t, int i) {
+  if constexpr (VEC) {
     const int c = (t + TPR * i) * 8;
     if (c < cols) {
-      unpack8(ldg8(row + c), v);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      r.q = __ldg(reinterpret_cast<const uint2*>(codes + c));
+      r.ex = __ldg(exps + (c >> 5));
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = col_of<false, TPR>(t, i, j);
-      v[j] = c < cols ? ldg1(row + c) : 0.f;
+      if (c < cols) r.v[j] = fmul((float)__ldg(codes + c), act8_scale(__ldg(exps + (c >> 5))));
     }
   }
 }
-template <bool VEC, int TPR>
-__device__ __forceinline__ void load_chunk8(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps, int cols,
-                                            int t, int i, float (&v)[8]) {
-  if (VEC) {
-    const int c = (t + TPR * i) * 8;
-    if (c < cols) {
-      const uint2 q = __ldg(reinterpret_cast<const uint2*>(codes + c));
-      const float s = act8_scale(__ldg(exps + (c >> 5)));
+// The values of a chunk, in pairs, times a factor that the returned number
+// includes: a checkpoint's codes come as whole numbers, their power of two in
+// the factor.
+template <class T, bool SRC8, bool VEC>
+__device__ __forceinline__ float values(const Raw<T, SRC8, VEC>& r, float factor, F2 (&v)[4]) {
+  if constexpr (VEC && SRC8) {
+    v[0] = act8_pair(r.q.x, 0);
+    v[1] = act8_pair(r.q.x, 1);
+    v[2] = act8_pair(r.q.y, 0);
+    v[3] = act8_pair(r.q.y, 1);
+    return factor * act8_scale(r.ex);
+  } else if constexpr (VEC) {
+    unpack8(r.q, v);
+  } else if constexpr (SRC8) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = act8_value(j < 4 ? q.x : q.y, j & 3, s);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    }
+    for (int j = 0; j < 4; ++j) v[j] = f2(r.v[2 * j], r.v[2 * j + 1]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = col_of<false, TPR>(t, i, j);
-      v[j] = c < cols ? fmul((float)codes[c], act8_scale(__ldg(exps + (c >> 5)))) : 0.f;
-    }
+    for (int j = 0; j < 4; ++j) v[j] = f2(Elem<T>::to_f(r.v[2 * j]), Elem<T>::to_f(r.v[2 * j + 1]));
   }
+  return factor;
 }
 template <class T, bool VEC, int TPR>
-__device__ __forceinline__ void load_param(const void* p, int f32, int vec, int cols, int t, int i, float (&v)[8]) {
+__device__ __forceinline__ void load_param(const void* p, int f32, int vec, int cols, int t, int i, F2 (&v)[4]) {
   if (VEC && vec) {
-    if (f32)
-      load_chunk<float, true, TPR>((const float*)p, cols, t, i, v);
-    else
-      load_chunk<T, true, TPR>((const T*)p, cols, t, i, v);
+    const int c = (t + TPR * i) * 8;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = f2(0.f);
+    if (c < cols) {
+      if (f32)
+        unpack8(ldg8((const float*)p + c), v);
+      else
+        unpack8(ldg8((const T*)p + c), v);
+    }
   } else {
+    float u[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = col_of<VEC, TPR>(t, i, j);
-      v[j] = c >= cols ? 0.f : f32 ? __ldg((const float*)p + c) : ldg1((const T*)p + c);
+      u[j] = c >= cols ? 0.f : f32 ? __ldg((const float*)p + c) : ldg1((const T*)p + c);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = f2(u[2 * j], u[2 * j + 1]);
   }
 }
 template <class T, bool VEC, int TPR>
-__device__ __forceinline__ void store_chunk(T* __restrict__ row, int cols, int t, int i, const float (&v)[8]) {
+__device__ __forceinline__ void store_chunk(T* __restrict__ row, int cols, int t, int i, const F2 (&v)[4]) {
   if (VEC) {
     const int c = (t + TPR * i) * 8;
     if (c < cols) stg8(row + c, v);
   } else {
+    float u[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f2_split(v[j], u[2 * j], u[2 * j + 1]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = col_of<false, TPR>(t, i, j);
-      if (c < cols) row[c] = Elem<T>::from_f(v[j]);
+      if (c < cols) row[c] = Elem<T>::from_f(u[j]);
     }
   }
 }
 
-// Sums of a and b over the TPR threads of a row (a block is one row for
-// TPR > 32; the trailing barrier lets the scratch be used again).
+// Threads of a block: several rows at a time up to 256 threads, else one row.
 template <int TPR>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float* scratch) {
+__host__ __device__ constexpr int block_threads() { return TPR < 256 ? 256 : TPR; }
+template <int TPR>
+__host__ __device__ constexpr int rows_per_block() { return block_threads<TPR>() / TPR; }
+
+// Sums of a and b over the TPR threads of a row. Rows of several warps meet in
+// shared memory; consecutive calls of a row alternate between two halves of it,
+// so that one barrier per call is enough.
+struct Scratch {
+  float v[2][2][32];
+};
+template <int TPR>
+__device__ __forceinline__ void row_barrier() {
+  if (TPR >= 256)
+    __syncthreads();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / TPR), "n"(TPR) : "memory");
+}
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, Scratch& scratch, int& turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     a += __shfl_xor_sync(0xffffffffu, a, o);
@@ -129,20 +193,23 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* scratch) {
   }
   if (TPR > 32) {
     constexpr int W = TPR / 32;
-    const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int w = threadIdx.x >> 5, l = threadIdx.x & 31, w0 = w / W * W;
+    float(&s)[2][32] = scratch.v[turn];
+    turn ^= 1;
     if (l == 0) {
-      scratch[w] = a;
-      scratch[32 + w] = b;
+      s[0][w] = a;
+      s[1][w] = b;
     }
-    __syncthreads();
-    a = l < W ? scratch[l] : 0.f;
-    b = l < W ? scratch[32 + l] : 0.f;
+    row_barrier<TPR>();
+    a = l < W ? s[0][w0 + l] : 0.f;
+    b = l < W ? s[1][w0 + l] : 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = W / 2; o > 0; o >>= 1) {
       a += __shfl_xor_sync(0xffffffffu, a, o);
       b += __shfl_xor_sync(0xffffffffu, b, o);
     }
-    __syncthreads();
+    a = __shfl_sync(0xffffffffu, a, 0);
+    b = __shfl_sync(0xffffffffu, b, 0);
   }
 }
 
@@ -150,7 +217,7 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* scratch) {
 // neighbouring threads' chunks (VEC) or the same element of a warp's lanes.
 template <class T, bool VEC, int TPR>
 __device__ __forceinline__ void store_act8(int8_t* __restrict__ codes, uint8_t* __restrict__ exps, int cols, int t, int i,
-                                           const float (&v)[8], bool live) {
+                                           const float (&v)[8]) {
   if (VEC) {
     uint32_t top = 0;
 #pragma unroll
@@ -160,7 +227,7 @@ __device__ __forceinline__ void store_act8(int8_t* __restrict__ codes, uint8_t* 
     const uint32_t byte = act8_exponent(top, act8_floor<T>());
     const float inv = act8_inverse(byte);
     const int c = (t + TPR * i) * 8;
-    if (!live || c >= cols) return;
+    if (c >= cols) return;
     const bool nan = byte == kAct8Nan;
     *reinterpret_cast<uint2*>(codes + c) =
         make_uint2(act8_codes4(v[0], v[1], v[2], v[3], inv, nan), act8_codes4(v[4], v[5], v[6], v[7], inv, nan));
@@ -171,7 +238,7 @@ __device__ __forceinline__ void store_act8(int8_t* __restrict__ codes, uint8_t* 
       const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7FFFFFFFu);
       const uint32_t byte = act8_exponent(top, act8_floor<T>());
       const int c = col_of<false, TPR>(t, i, j);
-      if (live && c < cols) {
+      if (c < cols) {
         codes[c] = (int8_t)act8_code(v[j], act8_inverse(byte), byte == kAct8Nan);
         if ((t & 31) == 0) exps[c >> 5] = (uint8_t)byte;
       }
@@ -179,154 +246,284 @@ __device__ __forceinline__ void store_act8(int8_t* __restrict__ codes, uint8_t* 
   }
 }
 
-template <int TPR>
-__host__ __device__ constexpr int block_threads() { return TPR == 32 ? 256 : TPR; }
-
 template <class T, bool VEC, int TPR, int NB>
 __global__ void __launch_bounds__(block_threads<TPR>()) forward_kernel(Args a) {
-  constexpr int RPB = block_threads<TPR>() / TPR;
-  __shared__ float scratch[64];
+  constexpr int RPB = rows_per_block<TPR>();
+  __shared__ Scratch scratch;
+  int turn = 0;
   const int t = threadIdx.x % TPR;
   const float inv_d = 1.f / (float)a.cols;
-  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB) {
-    const long long row = row0 + threadIdx.x / TPR;
-    const bool live = row < a.rows;
-    if (TPR == 32 && !live) return;  // whole warps
-    const T* src = (const T*)a.x + row * a.ldx;
-    float v[NB][8];
-    float s = 0.f, zero = 0.f;
+  const long long step = (long long)gridDim.x * RPB;
+  long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (row >= a.rows) return;  // whole row groups, which alone meet at barriers
+  Raw<T, false, VEC> next[NB] = {};  // columns past the row's end stay zero
+#pragma unroll
+  for (int i = 0; i < NB; ++i) fetch<T, VEC, TPR>(next[i], (const T*)a.x + row * a.ldx, a.cols, t, i);
+  for (; row < a.rows; row += step) {
+    F2 v[NB][4], acc = f2(0.f);
+    float zero = 0.f;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      load_chunk<T, VEC, TPR>(src, a.cols, t, i, v[i]);
+      values<T, false, VEC>(next[i], 1.f, v[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += v[i][j];
+      for (int j = 0; j < 4; ++j) acc = add2(acc, v[i][j]);
     }
-    row_sum2<TPR>(s, zero, scratch);
+    if (row + step < a.rows) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) fetch<T, VEC, TPR>(next[i], (const T*)a.x + (row + step) * a.ldx, a.cols, t, i);
+    }
+    float s = f2_sum(acc);
+    row_sum2<TPR>(s, zero, scratch, turn);
     const float mean = s * inv_d;
-    float q = 0.f;
+    const F2 minus = f2(-mean);
+    if (a.codes_out) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+      for (int i = 0; i < NB; ++i) {
+        float u[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float u = col_of<VEC, TPR>(t, i, j) < a.cols ? v[i][j] - mean : 0.f;
-        q = fmaf(u, u, q);
+        for (int j = 0; j < 4; ++j) f2_split(v[i][j], u[2 * j], u[2 * j + 1]);
+        store_act8<T, VEC, TPR>(a.codes_out + row * a.cols, a.exps_out + row * act8_blocks(a.cols), a.cols, t, i, u);
       }
-    row_sum2<TPR>(q, zero, scratch);
+    }
+    acc = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = add2(v[i][j], minus);
+      if (VEC) {
+        if (col_of<VEC, TPR>(t, i, 0) < a.cols) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc = fma2(v[i][j], v[i][j], acc);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float lo, hi;
+          f2_split(v[i][j], lo, hi);
+          lo = col_of<VEC, TPR>(t, i, 2 * j) < a.cols ? lo : 0.f;
+          hi = col_of<VEC, TPR>(t, i, 2 * j + 1) < a.cols ? hi : 0.f;
+          acc = fma2(f2(lo, hi), f2(lo, hi), acc);
+        }
+      }
+    }
+    float q = f2_sum(acc);
+    row_sum2<TPR>(q, zero, scratch, turn);
     const float rstd = 1.f / sqrtf(q * inv_d + a.eps);
     if (t == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
     }
-    if (a.codes_out) {
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-        store_act8<T, VEC, TPR>(a.codes_out + row * a.cols, a.exps_out + row * act8_blocks(a.cols), a.cols, t, i, v[i], true);
-    }
+    const F2 scale = f2(rstd);
     T* dst = (T*)a.out + row * a.ldo;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      float w[8], b[8], y[8];
+      F2 w[4], b[4], y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = f2(1.f);
+        b[j] = f2(0.f);
+      }
       if (a.weight) load_param<T, VEC, TPR>(a.weight, a.w_f32, a.w_vec, a.cols, t, i, w);
       if (a.bias) load_param<T, VEC, TPR>(a.bias, a.w_f32, a.w_vec, a.cols, t, i, b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float h = (v[i][j] - mean) * rstd;
-        if (a.weight) h *= w[j];
-        if (a.bias) h += b[j];
-        y[j] = h;
-      }
+      for (int j = 0; j < 4; ++j) y[j] = fma2(mul2(v[i][j], scale), w[j], b[j]);
       store_chunk<T, VEC, TPR>(dst, a.cols, t, i, y);
     }
   }
 }
 
+// Rows on their way ahead of the one being worked on. One row per row group did
+// not cover the memory's latency (8192 x 8192: 24 KB in flight per SM, 2.6 TB/s),
+// so where rows can be read 16 bytes at a time every thread copies its own
+// chunks of the next rows into shared memory asynchronously (no barrier: nobody
+// else reads them); other rows come one ahead through registers.
+template <class T, bool SRC8, int TPR, int NB>
+struct Ring {
+  static constexpr int DY = sizeof(T) / 2, X = SRC8 ? 1 : sizeof(T) / 2;  // 16-byte slots per chunk (8 bytes of codes take one)
+  static constexpr int SLOTS = NB * (DY + X);
+  static constexpr int TH = block_threads<TPR>();
+  static constexpr int BLOCKS = TH == 256 ? 2 : 1;  // per SM, at 128 registers per thread
+  static constexpr int DEPTH = 3;
+  static constexpr int BYTES = DEPTH * SLOTS * 16 * TH;
+};
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+template <class T, bool SRC8, bool VEC, int TPR>
+__device__ __forceinline__ void fetch_x(const Args& a, Raw<T, SRC8, VEC>& r, long long row, int t, int i) {
+  if constexpr (SRC8)
+    fetch8<T, VEC, TPR>(r, a.codes + row * a.cols, a.exps + row * act8_blocks(a.cols), a.cols, t, i);
+  else
+    fetch<T, VEC, TPR>(r, (const T*)a.x + row * a.ldx, a.cols, t, i);
+}
 template <class T, bool SRC8, bool VEC, int TPR, int NB>
-__global__ void __launch_bounds__(block_threads<TPR>()) backward_kernel(Args a) {
-  constexpr int THREADS = block_threads<TPR>();
-  constexpr int RPB = THREADS / TPR;
-  __shared__ float scratch[RPB > 1 ? RPB * 256 : 64];
+__global__ void __launch_bounds__(block_threads<TPR>(), Ring<T, SRC8, TPR, NB>::BLOCKS)
+    backward_kernel(Args a) {
+  using R = Ring<T, SRC8, TPR, NB>;
+  constexpr int RPB = rows_per_block<TPR>(), TH = R::TH;
+  extern __shared__ uint4 ring[];
+  __shared__ Scratch scratch;
+  __shared__ float sums[RPB > 1 ? 8 : 1][256];
+  int turn = 0;
   const int t = threadIdx.x % TPR;
   const float inv_d = 1.f / (float)a.cols;
-  float dw[NB][8], db[NB][8];
+  const long long step = (long long)gridDim.x * RPB;
+  long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  F2 dw[NB][4], db[NB][4], w[NB][4];
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int i = 0; i < NB; ++i) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.f;
-  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB) {
-    const long long row = row0 + threadIdx.x / TPR;
-    if (TPR == 32 && row >= a.rows) break;  // whole warps; no block barrier in the loop
-    const float mean = __ldg(a.mean + row), rstd = __ldg(a.rstd + row);
-    float xh[NB][8], g[NB][8];
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      if (SRC8)
-        load_chunk8<VEC, TPR>(a.codes + row * a.cols, a.exps + row * act8_blocks(a.cols), a.cols, t, i, xh[i]);
-      else
-        load_chunk<T, VEC, TPR>((const T*)a.x + row * a.ldx, a.cols, t, i, xh[i]);
-      load_chunk<T, VEC, TPR>((const T*)a.dy + row * a.ldy, a.cols, t, i, g[i]);
+    for (int j = 0; j < 4; ++j) {
+      dw[i][j] = db[i][j] = f2(0.f);
+      w[i][j] = f2(1.f);
     }
+    if (a.weight) load_param<T, VEC, TPR>(a.weight, a.w_f32, a.w_vec, a.cols, t, i, w[i]);
+  }
+  // columns past the row's end are zero, and with them their part of every sum
+  Raw<T, SRC8, VEC> next_x[VEC ? 1 : NB] = {};
+  Raw<T, false, VEC> next_dy[VEC ? 1 : NB] = {};
+  uint32_t next_ex[NB] = {};
+  float next_mean = 0.f, next_rstd = 0.f;
+  // what comes through registers, a row ahead
+  auto fetch_row = [&](long long r) {
+    next_mean = __ldg(a.mean + r);
+    next_rstd = __ldg(a.rstd + r);
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      float w[8];
-      if (a.weight) load_param<T, VEC, TPR>(a.weight, a.w_f32, a.w_vec, a.cols, t, i, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (col_of<VEC, TPR>(t, i, j) < a.cols) {
-          const float h = (xh[i][j] - mean) * rstd, d = g[i][j];
-          dw[i][j] = fmaf(d, h, dw[i][j]);
-          db[i][j] += d;
-          const float gg = a.weight ? d * w[j] : d;
-          s1 += gg;
-          s2 = fmaf(gg, h, s2);
-          xh[i][j] = h;
-          g[i][j] = gg;
-        }
+      if constexpr (VEC) {
+        const int c = (t + TPR * i) * 8;
+        if (SRC8 && c < a.cols) next_ex[i] = __ldg(a.exps + r * act8_blocks(a.cols) + (c >> 5));
+      } else {
+        fetch_x<T, SRC8, VEC, TPR>(a, next_x[i], r, t, i);
+        fetch<T, VEC, TPR>(next_dy[i], (const T*)a.dy + r * a.ldy, a.cols, t, i);
       }
     }
-    row_sum2<TPR>(s1, s2, scratch);
-    const float m1 = s1 * inv_d, m2 = s2 * inv_d;
+  };
+  // what comes through shared memory, stage s
+  auto copy_row = [&](long long r, int s) {
+    if constexpr (VEC) {
+      if (r < a.rows) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int c = (t + TPR * i) * 8;
+          if (c >= a.cols) continue;
+          uint4* slot = ring + ((size_t)s * R::SLOTS + i * (R::DY + R::X)) * TH + threadIdx.x;
+          const char* dy = (const char*)((const T*)a.dy + r * a.ldy + c);
+#pragma unroll
+          for (int q = 0; q < R::DY; ++q) copy_async16(slot + q * TH, dy + 16 * q);
+          slot += R::DY * TH;
+          if constexpr (SRC8) {
+            copy_async8(slot, a.codes + r * a.cols + c);
+          } else {
+            const char* x = (const char*)((const T*)a.x + r * a.ldx + c);
+#pragma unroll
+            for (int q = 0; q < R::X; ++q) copy_async16(slot + q * TH, x + 16 * q);
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  int stage = 0;
+  if (row < a.rows) fetch_row(row);
+#pragma unroll
+  for (int s = 0; s < R::DEPTH - 1; ++s) copy_row(row + s * step, s);
+  for (; row < a.rows; row += step) {  // whole row groups, which alone meet at barriers
+    const float mean = next_mean, rstd = next_rstd;
+    // xh = x rstd - mean rstd, a checkpoint's scale within the factor
+    const float shift = -mean * rstd;
+    F2 h[NB][4], g[NB][4];
+    float factor[NB];
+    if constexpr (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(R::DEPTH - 2) : "memory");
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      if constexpr (VEC) {
+        Raw<T, SRC8, VEC> x = {};
+        Raw<T, false, VEC> dy = {};
+        if ((t + TPR * i) * 8 < a.cols) {
+          const uint4* slot = ring + (stage * R::SLOTS + i * (R::DY + R::X)) * TH + threadIdx.x;
+#pragma unroll
+          for (int q = 0; q < R::DY; ++q) dy.q.q[q] = slot[q * TH];
+          slot += R::DY * TH;
+          if constexpr (SRC8) {
+            x.q = *reinterpret_cast<const uint2*>(slot);
+            x.ex = next_ex[i];
+          } else {
+#pragma unroll
+            for (int q = 0; q < R::X; ++q) x.q.q[q] = slot[q * TH];
+          }
+        }
+        factor[i] = values<T, SRC8, VEC>(x, rstd, h[i]);
+        values<T, false, VEC>(dy, 1.f, g[i]);
+      } else {
+        factor[i] = values<T, SRC8, VEC>(next_x[i], rstd, h[i]);
+        values<T, false, VEC>(next_dy[i], 1.f, g[i]);
+      }
+    }
+    copy_row(row + (R::DEPTH - 1) * step, stage == 0 ? R::DEPTH - 1 : stage - 1);  // the stage read last
+    if (row + step < a.rows) fetch_row(row + step);
+    F2 acc1 = f2(0.f), acc2 = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        h[i][j] = fma2(h[i][j], f2(factor[i]), f2(shift));
+        dw[i][j] = fma2(g[i][j], h[i][j], dw[i][j]);
+        db[i][j] = add2(db[i][j], g[i][j]);
+        g[i][j] = mul2(g[i][j], w[i][j]);
+        acc1 = add2(acc1, g[i][j]);
+        acc2 = fma2(g[i][j], h[i][j], acc2);
+      }
+    float s1 = f2_sum(acc1), s2 = f2_sum(acc2);
+    row_sum2<TPR>(s1, s2, scratch, turn);
+    const F2 m1 = f2(-s1 * inv_d * rstd), m2 = f2(-s2 * inv_d * rstd), scale = f2(rstd);
     T* dst = (T*)a.out + row * a.ldo;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      float d[8];
+      F2 d[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = rstd * (g[i][j] - m1 - xh[i][j] * m2);
+      for (int j = 0; j < 4; ++j) d[j] = fma2(h[i][j], m2, fma2(g[i][j], scale, m1));
       store_chunk<T, VEC, TPR>(dst, a.cols, t, i, d);
     }
+    stage = stage + 1 == R::DEPTH ? 0 : stage + 1;
   }
   if (!a.part) return;
   float* part = a.part + (size_t)blockIdx.x * 2 * a.cols;
-  if (RPB == 1) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+  for (int i = 0; i < NB; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = col_of<VEC, TPR>(t, i, j);
-        if (c < a.cols) {
-          part[c] = dw[i][j];
-          part[a.cols + c] = db[i][j];
+    for (int k = 0; k < 2; ++k) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f2_split(k ? db[i][j] : dw[i][j], v[2 * j], v[2 * j + 1]);
+      float* row_k = part + (size_t)k * a.cols;
+      if (RPB == 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = col_of<VEC, TPR>(t, i, j);
+          if (c < a.cols) row_k[c] = v[j];
+        }
+      } else {
+        // the block's row groups hold the same columns: through shared memory,
+        // added in the groups' order
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[j][threadIdx.x] = v[j];
+        __syncthreads();
+        for (int o = threadIdx.x; o < 8 * TPR; o += 256) {
+          const int u = VEC ? o >> 3 : o % TPR, j = VEC ? o & 7 : o / TPR;  // neighbouring columns
+          float s = 0.f;
+#pragma unroll
+          for (int r = 0; r < RPB; ++r) s += sums[j][r * TPR + u];
+          const int c = col_of<VEC, TPR>(u, i, j);
+          if (c < a.cols) row_k[c] = s;
         }
       }
-  } else {
-    // the block's warps hold the same columns of different rows: one chunk of
-    // 256 columns at a time through shared memory, added in warp order
-    const int w = threadIdx.x / TPR;
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) scratch[w * 256 + j * 32 + t] = k ? db[i][j] : dw[i][j];
-        __syncthreads();
-        float s = 0.f;
-#pragma unroll
-        for (int r = 0; r < RPB; ++r) s += scratch[r * 256 + threadIdx.x];
-        const int c = col_of<VEC, TPR>(threadIdx.x & 31, i, threadIdx.x >> 5);
-        if (c < a.cols) part[(size_t)k * a.cols + c] = s;
-      }
-  }
+    }
 }
 
 // out_k[c] = sum over p of part[p][k][c]: 32 strands of p per column, each in
@@ -352,7 +549,7 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restric
   if (lx == 0 && blockIdx.x * 32 + ly < cols) out[blockIdx.x * 32 + ly] = Elem<W>::from_f(v);
 }
 
-// Rows longer than kMaxFused: one block per row, the row read once per pass.
+// Rows longer than that: one block per row, the row read once per pass.
 template <class T>
 __device__ __forceinline__ float load_any(const void* p, int f32, long long i) {
   return f32 ? __ldg((const float*)p + i) : ldg1((const T*)p + i);
@@ -365,19 +562,20 @@ __device__ __forceinline__ float load_x(const Args& a, long long row, int c) {
 }
 template <class T>
 __global__ void __launch_bounds__(1024) forward_long_kernel(Args a) {
-  __shared__ float scratch[64];
+  __shared__ Scratch scratch;
+  int turn = 0;
   const long long row = blockIdx.x;
   const float inv_d = 1.f / (float)a.cols;
   float s = 0.f, zero = 0.f;
   for (int c = threadIdx.x; c < a.cols; c += 1024) s += load_x<T, false>(a, row, c);
-  row_sum2<1024>(s, zero, scratch);
+  row_sum2<1024>(s, zero, scratch, turn);
   const float mean = s * inv_d;
   float q = 0.f;
   for (int c = threadIdx.x; c < a.cols; c += 1024) {
     const float u = load_x<T, false>(a, row, c) - mean;
     q = fmaf(u, u, q);
   }
-  row_sum2<1024>(q, zero, scratch);
+  row_sum2<1024>(q, zero, scratch, turn);
   const float rstd = 1.f / sqrtf(q * inv_d + a.eps);
   if (threadIdx.x == 0) {
     if (a.mean) a.mean[row] = mean;
@@ -395,16 +593,15 @@ __global__ void __launch_bounds__(1024) forward_long_kernel(Args a) {
       }
     }
     if (c < a.cols) {
-      float h = (x - mean) * rstd;
-      if (a.weight) h *= load_any<T>(a.weight, a.w_f32, c);
-      if (a.bias) h += load_any<T>(a.bias, a.w_f32, c);
-      ((T*)a.out)[row * a.ldo + c] = Elem<T>::from_f(h);
+      const float w = a.weight ? load_any<T>(a.weight, a.w_f32, c) : 1.f, b = a.bias ? load_any<T>(a.bias, a.w_f32, c) : 0.f;
+      ((T*)a.out)[row * a.ldo + c] = Elem<T>::from_f(fmaf(fmul(x - mean, rstd), w, b));
     }
   }
 }
 template <class T, bool SRC8>
 __global__ void __launch_bounds__(1024) backward_long_kernel(Args a) {
-  __shared__ float scratch[64];
+  __shared__ Scratch scratch;
+  int turn = 0;
   const long long row = blockIdx.x;
   const float inv_d = 1.f / (float)a.cols, mean = a.mean[row], rstd = a.rstd[row];
   const T* dy = (const T*)a.dy + row * a.ldy;
@@ -416,7 +613,7 @@ __global__ void __launch_bounds__(1024) backward_long_kernel(Args a) {
     s1 += g;
     s2 = fmaf(g, h, s2);
   }
-  row_sum2<1024>(s1, s2, scratch);
+  row_sum2<1024>(s1, s2, scratch, turn);
   const float m1 = s1 * inv_d, m2 = s2 * inv_d;
   for (int c = threadIdx.x; c < a.cols; c += 1024) {
     const float h = (load_x<T, SRC8>(a, row, c) - mean) * rstd;
@@ -444,50 +641,65 @@ __global__ void __launch_bounds__(256) weight_grad_long_kernel(Args a) {
 struct Shape {
   int tpr, nb;
 };
-// Threads and chunks of eight columns per thread that hold a row.
+// Threads and chunks of eight columns per thread that hold a row: at most two
+// chunks, whose sums of dw and db fit the registers beside the next row, but for
+// the widest rows.
 static Shape shape_for(int cols) {
   const int chunks = cdiv(cols, 8);
-  if (chunks <= 128) return {32, chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4};
-  if (chunks <= 256) return {128, 2};
-  if (chunks <= 512) return {256, 2};
-  if (chunks <= 1024) return {512, 2};
+  if (chunks <= 32) return {32, 1};
+  for (int tpr = 32; tpr <= 512; tpr *= 2)
+    if (chunks <= 2 * tpr) return {tpr, 2};
   return {512, 4};
 }
-// Blocks of the backward pass: enough to fill the SMs, and no more partial
-// rows of dw and db than that.
-static int backward_blocks(long long rows, int cols) {
-  if (cols > kMaxFused) return (int)(rows < 16 ? rows : 16);
+static int rows_per_block_of(int tpr) { return tpr < 256 ? 256 / tpr : 1; }
+// Blocks of the backward pass: as many as the SMs hold, and for short inputs at
+// least two rows per row group, since every block leaves a partial row of dw and
+// db to be read again.
+static int backward_blocks(int dtype, long long rows, int cols) {
+  if (cols > kMaxBackward) return (int)(rows < 16 ? rows : 16);
   const Shape s = shape_for(cols);
-  const int rpb = s.tpr == 32 ? 8 : 1;
-  const long long want = (rows + rpb - 1) / rpb;
-  const int per_sm = s.tpr <= 128 ? 4 : s.tpr == 256 ? 2 : 1;
-  return (int)(want < 148LL * per_sm ? want : 148LL * per_sm);
+  const int rpb = rows_per_block_of(s.tpr);
+  const long long want = (rows + 2 * rpb - 1) / (2 * rpb);
+  const long long most = 148 * (s.tpr <= 256 ? 2 : 1);
+  return (int)(want < most ? (want > 0 ? want : 1) : most);
 }
 
 template <class F>
 static void with_shape(Shape s, F&& f) {
 #define SCMP_SHAPE(T_, N_) \
   if (s.tpr == T_ && s.nb == N_) return f(std::integral_constant<int, T_>{}, std::integral_constant<int, N_>{});
-  SCMP_SHAPE(32, 1) SCMP_SHAPE(32, 2) SCMP_SHAPE(32, 4) SCMP_SHAPE(128, 2) SCMP_SHAPE(256, 2) SCMP_SHAPE(512, 2)
+  SCMP_SHAPE(32, 1) SCMP_SHAPE(32, 2) SCMP_SHAPE(64, 2) SCMP_SHAPE(128, 2) SCMP_SHAPE(256, 2) SCMP_SHAPE(512, 2)
   SCMP_SHAPE(512, 4)
 #undef SCMP_SHAPE
 }
 
+template <class K>
+static int blocks_per_sm(K kern, int threads) {
+  int n = 1;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) == cudaSuccess && n > 0 ? n : 1;
+}
 static cudaError_t launch_forward(const Args& a, int dtype, bool vec, cudaStream_t st) {
   with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    if (a.cols > kMaxFused) {
+    if (a.cols > kMaxForward) {
       forward_long_kernel<T><<<(unsigned)a.rows, 1024, 0, st>>>(a);
       return;
     }
     with_shape(shape_for(a.cols), [&](auto tpr, auto nb) {
       constexpr int TPR = decltype(tpr)::value, NB = decltype(nb)::value, TH = block_threads<TPR>();
+      // as many blocks as the SMs hold, each with its next row on the way
       const long long blocks = (a.rows + TH / TPR - 1) / (TH / TPR);
-      const int grid = (int)(blocks < (1 << 30) ? blocks : 1 << 30);
-      if (vec)
-        forward_kernel<T, true, TPR, NB><<<grid, TH, 0, st>>>(a);
-      else
-        forward_kernel<T, false, TPR, NB><<<grid, TH, 0, st>>>(a);
+      auto go = [&](auto kern, int per_sm) {
+        const int grid = (int)(blocks < 148LL * per_sm ? blocks : 148LL * per_sm);
+        kern<<<grid, TH, 0, st>>>(a);
+      };
+      if (vec) {
+        static const int per_sm = blocks_per_sm(forward_kernel<T, true, TPR, NB>, TH);
+        go(forward_kernel<T, true, TPR, NB>, per_sm);
+      } else {
+        static const int per_sm = blocks_per_sm(forward_kernel<T, false, TPR, NB>, TH);
+        go(forward_kernel<T, false, TPR, NB>, per_sm);
+      }
     });
   });
   count_launch();
@@ -499,7 +711,7 @@ static cudaError_t launch_backward(const Args& a, int dtype, bool vec, int block
     using T = std::remove_pointer_t<decltype(tag)>;
     auto go = [&](auto src8) {
       constexpr bool S8 = decltype(src8)::value;
-      if (a.cols > kMaxFused) {
+      if (a.cols > kMaxBackward) {
         backward_long_kernel<T, S8><<<(unsigned)a.rows, 1024, 0, st>>>(a);
         if (a.part) {
           weight_grad_long_kernel<T, S8><<<dim3(cdiv(a.cols, 256), blocks), 256, 0, st>>>(a);
@@ -508,11 +720,14 @@ static cudaError_t launch_backward(const Args& a, int dtype, bool vec, int block
         return;
       }
       with_shape(shape_for(a.cols), [&](auto tpr, auto nb) {
-        constexpr int TPR = decltype(tpr)::value, NB = decltype(nb)::value, TH = block_threads<TPR>();
-        if (vec)
-          backward_kernel<T, S8, true, TPR, NB><<<blocks, TH, 0, st>>>(a);
-        else
+        constexpr int TPR = decltype(tpr)::value, NB = decltype(nb)::value > 2 ? 2 : decltype(nb)::value, TH = block_threads<TPR>();
+        if (vec) {
+          constexpr int smem = Ring<T, S8, TPR, NB>::BYTES;
+          cudaFuncSetAttribute(backward_kernel<T, S8, true, TPR, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+          backward_kernel<T, S8, true, TPR, NB><<<blocks, TH, smem, st>>>(a);
+        } else {
           backward_kernel<T, S8, false, TPR, NB><<<blocks, TH, 0, st>>>(a);
+        }
       });
     };
     if (a.codes)
@@ -570,10 +785,10 @@ int scmp_layer_norm_forward(const void* x, int dtype, long long rows, int cols, 
   return SCMP_OK;
 }
 
-int scmp_layer_norm_backward_workspace_size(long long rows, int cols, size_t* bytes) {
-  if (rows < 0 || rows >= (1LL << 31) || cols < 1 || !bytes)
+int scmp_layer_norm_backward_workspace_size(int dtype, long long rows, int cols, size_t* bytes) {
+  if (!dtype_ok(dtype) || rows < 0 || rows >= (1LL << 31) || cols < 1 || !bytes)
     return fail(SCMP_ERR_INVALID_ARG, "layer_norm_backward_workspace_size: bad arguments");
-  *bytes = (size_t)ln::backward_blocks(rows, cols) * 2 * cols * sizeof(float);
+  *bytes = (size_t)ln::backward_blocks(dtype, rows, cols) * 2 * cols * sizeof(float);
   return SCMP_OK;
 }
 
@@ -592,7 +807,7 @@ int scmp_layer_norm_backward(const void* dy, long long lddy, const void* x, long
   if (!x == !codes || !codes != !exps)
     return fail(SCMP_ERR_INVALID_ARG, "layer_norm_backward: give x, or codes and exps");
   if (!dy || !mean || !rstd || !dx) return fail(SCMP_ERR_INVALID_ARG, "layer_norm_backward: null pointer");
-  const int blocks = ln::backward_blocks(rows, cols);
+  const int blocks = ln::backward_blocks(dtype, rows, cols);
   const bool sums = dweight || dbias;
   if (sums && (!workspace || workspace_bytes < (size_t)blocks * 2 * cols * sizeof(float)))
     return fail(SCMP_ERR_WORKSPACE, "layer_norm_backward: workspace missing or too small");

@@ -816,12 +816,14 @@ static cudaError_t launch_tc(const Operand& a, const Operand& b, long long m, in
 // Rows at a 16-byte pitch; a float32 matrix as three bfloat16 planes (split3).
 template <class T>
 __global__ void __launch_bounds__(256) restage_kernel(const T* __restrict__ x, long long rows, int cols, long long ld,
-                                                      uint16_t* __restrict__ out, long long ldo, bool vec) {
+                                                      uint16_t* __restrict__ out, long long ldo, bool vec, FastDiv by) {
   const int oct = cdiv(cols, 8);
   const long long total = rows * oct, plane = rows * ldo;
   for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
-    const long long row = t / oct;
-    const int c = (int)(t - row * oct) * 8;
+    long long row;
+    int c;
+    row_and_piece(t, by, total < 1LL << 31, row, c);
+    c *= 8;
     const T* src = x + row * ld + c;
     uint16_t* dst = out + row * ldo + c;
     if constexpr (sizeof(T) == 2) {
@@ -856,9 +858,9 @@ static cudaError_t launch_restage(const void* x, long long rows, int cols, long 
   const long long items = rows * cdiv(cols, 8);
   const int grid = (int)((items + 255) / 256 < 148 * 8 ? (items + 255) / 256 : 148 * 8);
   if (dtype == SCMP_F32)
-    restage_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, cols, ld, (uint16_t*)out, pitch_of(cols), rows_aligned16(x, ld, 4));
+    restage_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, cols, ld, (uint16_t*)out, pitch_of(cols), rows_aligned16(x, ld, 4), FastDiv(cdiv(cols, 8)));
   else
-    restage_kernel<__half><<<grid, 256, 0, st>>>((const __half*)x, rows, cols, ld, (uint16_t*)out, pitch_of(cols), false);
+    restage_kernel<__half><<<grid, 256, 0, st>>>((const __half*)x, rows, cols, ld, (uint16_t*)out, pitch_of(cols), false, FastDiv(cdiv(cols, 8)));
   count_launch();
   return cudaGetLastError();
 }

@@ -47,13 +47,17 @@ static auto with_dtype(int dtype, F&& f) {
 // integers: the 16-bit types' own __ldg is an asm statement without side
 // effects, which the compiler may run before the condition that guards it.
 template <class T>
-__device__ __forceinline__ float ldg1(const T* p) {
+__device__ __forceinline__ T ldg_raw(const T* p) {
   if constexpr (sizeof(T) == 2) {
     const unsigned short u = __ldg(reinterpret_cast<const unsigned short*>(p));
-    return Elem<T>::to_f(*reinterpret_cast<const T*>(&u));
+    return *reinterpret_cast<const T*>(&u);
   } else {
     return __ldg(p);
   }
+}
+template <class T>
+__device__ __forceinline__ float ldg1(const T* p) {
+  return Elem<T>::to_f(ldg_raw(p));
 }
 
 // Eight consecutive values as they lie in memory (16 or 32 bytes, 16-byte aligned).
@@ -121,6 +125,102 @@ __device__ __forceinline__ void stg4(T* p, const float (&v)[4]) {
     *reinterpret_cast<uint2*>(p) = make_uint2(pack2(v[0], v[1], p), pack2(v[2], v[3], p));
   else
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// Two float32 per instruction (each half an IEEE operation of its own). The
+// row-wise kernels are bound by instruction issue as much as by memory.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
+__device__ __forceinline__ void f2_split(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float f2_sum(F2 a) {
+  float lo, hi;
+  f2_split(a, lo, hi);
+  return lo + hi;
+}
+// The two values of a word of 16-bit ones.
+__device__ __forceinline__ F2 unpack_pair(uint32_t w, const __nv_bfloat16*) {
+  return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ F2 unpack_pair(uint32_t w, const __half*) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f2(f.x, f.y);
+}
+template <class T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, F2 (&v)[4]) {
+  if constexpr (sizeof(T) == 2) {
+    v[0] = unpack_pair(r.q[0].x, (const T*)nullptr);
+    v[1] = unpack_pair(r.q[0].y, (const T*)nullptr);
+    v[2] = unpack_pair(r.q[0].z, (const T*)nullptr);
+    v[3] = unpack_pair(r.q[0].w, (const T*)nullptr);
+  } else {
+    const float* e = reinterpret_cast<const float*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f2(e[2 * i], e[2 * i + 1]);
+  }
+}
+__device__ __forceinline__ uint32_t pack_pair(F2 a, const __nv_bfloat16* t) {
+  float lo, hi;
+  f2_split(a, lo, hi);
+  return pack2(lo, hi, t);
+}
+__device__ __forceinline__ uint32_t pack_pair(F2 a, const __half* t) {
+  float lo, hi;
+  f2_split(a, lo, hi);
+  return pack2(lo, hi, t);
+}
+template <class T>
+__device__ __forceinline__ void stg8(T* p, const F2 (&v)[4]) {
+  if constexpr (sizeof(T) == 2) {
+    const T* t = nullptr;
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_pair(v[0], t), pack_pair(v[1], t), pack_pair(v[2], t), pack_pair(v[3], t));
+  } else {
+    ulonglong2* d = reinterpret_cast<ulonglong2*>(p);
+    d[0] = make_ulonglong2(v[0].v, v[1].v);
+    d[1] = make_ulonglong2(v[2].v, v[3].v);
+  }
+}
+
+// Division of n < 2^31 by a number fixed at launch: (umulhi(n, mul) + n) >> shift.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  explicit FastDiv(uint32_t by = 1) : d(by), mul(0), shift(0) {
+    while (shift < 31 && (1u << shift) < by) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - by)) / by + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+// Index t into rows of d.d pieces: (row, piece).
+__device__ __forceinline__ void row_and_piece(long long t, const FastDiv& d, bool small, long long& row, int& piece) {
+  if (small) {
+    const uint32_t r = d.div((uint32_t)t);
+    row = r;
+    piece = (int)((uint32_t)t - r * d.d);
+  } else {
+    row = t / d.d;
+    piece = (int)(t - row * d.d);
+  }
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -43,8 +43,8 @@ def test_layer_norm_arguments():
     refused(bwd(P, 8, None, 0, None, None, 0, 1, 8, P, P, None, 0, P, None, None, None, 0, None), "codes")
     refused(bwd(P, 8, P, 8, P, P, 0, 1, 8, P, P, None, 0, P, None, None, None, 0, None), "codes")
     refused(bwd(P, 4, P, 8, None, None, 0, 1, 8, P, P, None, 0, P, None, None, None, 0, None), "pitch")
-    refused(lib.scmp_layer_norm_backward_workspace_size(4, 0, ctypes.byref(n)), "arguments")
-    assert lib.scmp_layer_norm_backward_workspace_size(0, 8, ctypes.byref(n)) == _lib.SCMP_OK
+    refused(lib.scmp_layer_norm_backward_workspace_size(0, 4, 0, ctypes.byref(n)), "arguments")
+    assert lib.scmp_layer_norm_backward_workspace_size(0, 0, 8, ctypes.byref(n)) == _lib.SCMP_OK
 
 
 def test_linear_arguments():
