@@ -30,6 +30,7 @@ UNITS = {
 }
 # Headers that only some units include.
 UNIT_HEADERS = {"internal.cuh": ("scmp_b200",), "quant.cuh": ("scmp_b200",), "vecio.cuh": ("norms", "linears"),
+                "launch.cuh": ("norms", "linears"),
                 "act8.cuh": ("norms", "linears"), "linear.cuh": ("linears",)}
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

@@ -1,5 +1,6 @@
 // Packing and unpacking of 8-bit activation checkpoints.
 #include "act8.cuh"
+#include "launch.cuh"
 #include "status.cuh"
 
 namespace scmp {
@@ -12,6 +13,8 @@ __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x,
   const int nb = act8_blocks(cols), lane = threadIdx.x & 31;
   const long long total = rows * nb;
   const bool small = total < 1LL << 31;
+  let_next_start();
+  prior_done();
   if constexpr (VEC) {
     constexpr int U = 2;
     const int quarter = threadIdx.x & 3;
@@ -86,6 +89,8 @@ template <class T, bool VEC>
 __global__ void __launch_bounds__(256) act8_unpack_kernel(const int8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
                                                           long long rows, int cols, long long ldo, T* __restrict__ out, FastDiv by) {
   const int nb = act8_blocks(cols);
+  let_next_start();
+  prior_done();
   if constexpr (VEC) {
     constexpr int PER = 16 / sizeof(T), U = 4;
     const int per_row = cols / PER;
@@ -151,15 +156,12 @@ cudaError_t launch_act8_unpack(const int8_t* codes, const uint8_t* exps, long lo
                                long long ldo, int dtype, cudaStream_t st) {
   const bool vec = cols % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && rows_aligned16(out, ldo, dtype_size(dtype));
   const int grid = elementwise_grid(rows * act8_blocks(cols) * 4, vec ? 256 : 32);
-  with_dtype(dtype, [&](auto* tag) {
+  return with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    if (vec)
-      act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, exps, rows, cols, ldo, (T*)out, FastDiv(cols / (16 / sizeof(T))));
-    else
-      act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, exps, rows, cols, ldo, (T*)out, FastDiv(act8_blocks(cols)));
+    const FastDiv by(vec ? cols / (16 / sizeof(T)) : act8_blocks(cols));
+    return launch_overlapped(vec ? act8_unpack_kernel<T, true> : act8_unpack_kernel<T, false>, grid, 256, 0, st, 1, codes, exps, rows, cols,
+                             ldo, (T*)out, by);
   });
-  count_launch();
-  return cudaGetLastError();
 }
 
 }  // namespace scmp
@@ -177,15 +179,12 @@ int scmp_act8_pack(const void* x, int dtype, long long rows, int cols, long long
   const cudaStream_t st = (cudaStream_t)stream;
   const bool vec = cols % 8 == 0 && rows_aligned16(x, ld, dtype_size(dtype)) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
   const int grid = elementwise_grid(rows * act8_blocks(cols) * 4, vec ? 256 : 32);
-  with_dtype(dtype, [&](auto* tag) {
+  const cudaError_t e = with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    if (vec)
-      act8_pack_kernel<T, true><<<grid, 256, 0, st>>>((const T*)x, rows, cols, ld, codes, exps, FastDiv(act8_blocks(cols)));
-    else
-      act8_pack_kernel<T, false><<<grid, 256, 0, st>>>((const T*)x, rows, cols, ld, codes, exps, FastDiv(act8_blocks(cols)));
+    return launch_overlapped(vec ? act8_pack_kernel<T, true> : act8_pack_kernel<T, false>, grid, 256, 0, st, 1, (const T*)x, rows, cols, ld,
+                             codes, exps, FastDiv(act8_blocks(cols)));
   });
-  count_launch();
-  SCMP_CUDA(cudaGetLastError(), "act8_pack");
+  SCMP_CUDA(e, "act8_pack");
   return SCMP_OK;
 }
 

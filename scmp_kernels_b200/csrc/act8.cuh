@@ -56,6 +56,37 @@ __device__ __forceinline__ uint32_t act8_codes4(float a, float b, float c, float
   const uint32_t hi = __byte_perm(act8_rounded(c, inverse), act8_rounded(d, inverse), 0x0040);
   return nan_block ? 0u : __byte_perm(lo, hi, 0x5410);
 }
+// 32 values' codes as eight words, a pair per element of v. The clamp to 127 acts
+// on blocks whose largest value rounds to 128 alone, one in two hundred, so it is
+// left to a branch.
+__device__ __forceinline__ void act8_codes32(const F2 (&v)[16], float top, uint32_t byte, uint32_t (&words)[8]) {
+  const bool nan = byte == kAct8Nan;
+  const float inv = act8_inverse(byte);
+  if (top * inv >= 127.5f) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      float a, b, c, d;
+      f2_split(v[2 * q], a, b);
+      f2_split(v[2 * q + 1], c, d);
+      words[q] = act8_codes4(a, b, c, d, inv, nan);
+    }
+  } else {
+    const F2 inv2 = f2(inv), magic = f2(12582912.f);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const F2 lo = fma2(v[2 * q], inv2, magic), hi = fma2(v[2 * q + 1], inv2, magic);
+      const uint32_t l = __byte_perm((uint32_t)lo.v, (uint32_t)(lo.v >> 32), 0x0040);
+      const uint32_t h = __byte_perm((uint32_t)hi.v, (uint32_t)(hi.v >> 32), 0x0040);
+      words[q] = nan ? 0u : __byte_perm(l, h, 0x5410);
+    }
+  }
+}
+// Larger magnitude of two, NaN if either is one.
+__device__ __forceinline__ float max_abs_nan(float top, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(x)));
+  return r;
+}
 // The value of byte i of a word of codes: the byte (offset by 128) becomes the
 // low mantissa bits of 2^23, which is then subtracted. Conversions from
 // integers would share the pipe of exp2 and reciprocal.

@@ -14,6 +14,7 @@
 // kernel adds in a fixed order: no atomics, the same bits every time. Rows too
 // long for registers take the three-pass kernels at the end.
 #include "act8.cuh"
+#include "launch.cuh"
 #include "status.cuh"
 
 namespace scmp {
@@ -171,11 +172,11 @@ __host__ __device__ constexpr int block_threads() { return TPR < 256 ? 256 : TPR
 template <int TPR>
 __host__ __device__ constexpr int rows_per_block() { return block_threads<TPR>() / TPR; }
 
-// Sums of a and b over the TPR threads of a row. Rows of several warps meet in
-// shared memory; consecutive calls of a row alternate between two halves of it,
-// so that one barrier per call is enough.
+// Sums of both halves of v over the TPR threads of a row. Rows of several warps
+// meet in shared memory; consecutive calls of a row alternate between two halves
+// of the scratch, so that one barrier per call is enough.
 struct Scratch {
-  float v[2][2][32];
+  F2 v[2][32];
 };
 template <int TPR>
 __device__ __forceinline__ void row_barrier() {
@@ -185,32 +186,22 @@ __device__ __forceinline__ void row_barrier() {
     asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / TPR), "n"(TPR) : "memory");
 }
 template <int TPR>
-__device__ __forceinline__ void row_sum2(float& a, float& b, Scratch& scratch, int& turn) {
+__device__ __forceinline__ F2 row_sum(F2 v, Scratch& scratch, int& turn) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
-  if (TPR > 32) {
+  for (int o = 16; o > 0; o >>= 1) v = add2(v, F2{__shfl_xor_sync(0xffffffffu, v.v, o)});
+  if constexpr (TPR > 32) {
     constexpr int W = TPR / 32;
-    const int w = threadIdx.x >> 5, l = threadIdx.x & 31, w0 = w / W * W;
-    float(&s)[2][32] = scratch.v[turn];
+    const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+    F2* s = scratch.v[turn];
     turn ^= 1;
-    if (l == 0) {
-      s[0][w] = a;
-      s[1][w] = b;
-    }
+    if (l == 0) s[w] = v;
     row_barrier<TPR>();
-    a = l < W ? s[0][w0 + l] : 0.f;
-    b = l < W ? s[1][w0 + l] : 0.f;
+    // lanes l, l + W, .. hold the same warp's sums: every lane ends with the total
+    v = s[w / W * W + (l & (W - 1))];
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
-    a = __shfl_sync(0xffffffffu, a, 0);
-    b = __shfl_sync(0xffffffffu, b, 0);
+    for (int o = W / 2; o > 0; o >>= 1) v = add2(v, F2{__shfl_xor_sync(0xffffffffu, v.v, o)});
   }
+  return v;
 }
 
 // 8-bit checkpoint of chunk i of a row: a block of 32 columns is four
@@ -255,13 +246,14 @@ __global__ void __launch_bounds__(block_threads<TPR>()) forward_kernel(Args a) {
   const float inv_d = 1.f / (float)a.cols;
   const long long step = (long long)gridDim.x * RPB;
   long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  let_next_start();
+  prior_done();
   if (row >= a.rows) return;  // whole row groups, which alone meet at barriers
   Raw<T, false, VEC> next[NB] = {};  // columns past the row's end stay zero
 #pragma unroll
   for (int i = 0; i < NB; ++i) fetch<T, VEC, TPR>(next[i], (const T*)a.x + row * a.ldx, a.cols, t, i);
   for (; row < a.rows; row += step) {
     F2 v[NB][4], acc = f2(0.f);
-    float zero = 0.f;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       values<T, false, VEC>(next[i], 1.f, v[i]);
@@ -272,9 +264,7 @@ __global__ void __launch_bounds__(block_threads<TPR>()) forward_kernel(Args a) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) fetch<T, VEC, TPR>(next[i], (const T*)a.x + (row + step) * a.ldx, a.cols, t, i);
     }
-    float s = f2_sum(acc);
-    row_sum2<TPR>(s, zero, scratch, turn);
-    const float mean = s * inv_d;
+    const float mean = f2_sum(row_sum<TPR>(acc, scratch, turn)) * inv_d;
     const F2 minus = f2(-mean);
     if (a.codes_out) {
 #pragma unroll
@@ -306,9 +296,7 @@ __global__ void __launch_bounds__(block_threads<TPR>()) forward_kernel(Args a) {
         }
       }
     }
-    float q = f2_sum(acc);
-    row_sum2<TPR>(q, zero, scratch, turn);
-    const float rstd = 1.f / sqrtf(q * inv_d + a.eps);
+    const float rstd = 1.f / sqrtf(f2_sum(row_sum<TPR>(acc, scratch, turn)) * inv_d + a.eps);
     if (t == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
@@ -373,6 +361,8 @@ __global__ void __launch_bounds__(block_threads<TPR>(), Ring<T, SRC8, TPR, NB>::
   const float inv_d = 1.f / (float)a.cols;
   const long long step = (long long)gridDim.x * RPB;
   long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  let_next_start();
+  prior_done();
   F2 dw[NB][4], db[NB][4], w[NB][4];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
@@ -478,8 +468,8 @@ __global__ void __launch_bounds__(block_threads<TPR>(), Ring<T, SRC8, TPR, NB>::
         acc1 = add2(acc1, g[i][j]);
         acc2 = fma2(g[i][j], h[i][j], acc2);
       }
-    float s1 = f2_sum(acc1), s2 = f2_sum(acc2);
-    row_sum2<TPR>(s1, s2, scratch, turn);
+    float s1, s2;
+    f2_split(row_sum<TPR>(f2(f2_sum(acc1), f2_sum(acc2)), scratch, turn), s1, s2);
     const F2 m1 = f2(-s1 * inv_d * rstd), m2 = f2(-s2 * inv_d * rstd), scale = f2(rstd);
     T* dst = (T*)a.out + row * a.ldo;
 #pragma unroll
@@ -535,6 +525,8 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restric
   const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lx, k = blockIdx.y;
   W* out = k ? out1 : out0;
+  let_next_start();
+  prior_done();
   if (!out) return;
   float v = 0.f;
   if (c < cols) {
@@ -564,19 +556,19 @@ template <class T>
 __global__ void __launch_bounds__(1024) forward_long_kernel(Args a) {
   __shared__ Scratch scratch;
   int turn = 0;
+  let_next_start();
+  prior_done();
   const long long row = blockIdx.x;
   const float inv_d = 1.f / (float)a.cols;
-  float s = 0.f, zero = 0.f;
+  float s = 0.f;
   for (int c = threadIdx.x; c < a.cols; c += 1024) s += load_x<T, false>(a, row, c);
-  row_sum2<1024>(s, zero, scratch, turn);
-  const float mean = s * inv_d;
+  const float mean = f2_sum(row_sum<1024>(f2(s, 0.f), scratch, turn)) * inv_d;
   float q = 0.f;
   for (int c = threadIdx.x; c < a.cols; c += 1024) {
     const float u = load_x<T, false>(a, row, c) - mean;
     q = fmaf(u, u, q);
   }
-  row_sum2<1024>(q, zero, scratch, turn);
-  const float rstd = 1.f / sqrtf(q * inv_d + a.eps);
+  const float rstd = 1.f / sqrtf(f2_sum(row_sum<1024>(f2(q, 0.f), scratch, turn)) * inv_d + a.eps);
   if (threadIdx.x == 0) {
     if (a.mean) a.mean[row] = mean;
     if (a.rstd) a.rstd[row] = rstd;
@@ -602,6 +594,8 @@ template <class T, bool SRC8>
 __global__ void __launch_bounds__(1024) backward_long_kernel(Args a) {
   __shared__ Scratch scratch;
   int turn = 0;
+  let_next_start();
+  prior_done();
   const long long row = blockIdx.x;
   const float inv_d = 1.f / (float)a.cols, mean = a.mean[row], rstd = a.rstd[row];
   const T* dy = (const T*)a.dy + row * a.ldy;
@@ -613,7 +607,7 @@ __global__ void __launch_bounds__(1024) backward_long_kernel(Args a) {
     s1 += g;
     s2 = fmaf(g, h, s2);
   }
-  row_sum2<1024>(s1, s2, scratch, turn);
+  f2_split(row_sum<1024>(f2(s1, s2), scratch, turn), s1, s2);
   const float m1 = s1 * inv_d, m2 = s2 * inv_d;
   for (int c = threadIdx.x; c < a.cols; c += 1024) {
     const float h = (load_x<T, SRC8>(a, row, c) - mean) * rstd;
@@ -626,6 +620,8 @@ __global__ void __launch_bounds__(1024) backward_long_kernel(Args a) {
 template <class T, bool SRC8>
 __global__ void __launch_bounds__(256) weight_grad_long_kernel(Args a) {
   const int c = blockIdx.x * 256 + threadIdx.x;
+  let_next_start();
+  prior_done();
   if (c >= a.cols) return;
   float dw = 0.f, db = 0.f;
   for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
@@ -664,10 +660,11 @@ static int backward_blocks(int dtype, long long rows, int cols) {
   return (int)(want < most ? (want > 0 ? want : 1) : most);
 }
 
-template <class F>
+template <bool FORWARD, class F>
 static void with_shape(Shape s, F&& f) {
-#define SCMP_SHAPE(T_, N_) \
-  if (s.tpr == T_ && s.nb == N_) return f(std::integral_constant<int, T_>{}, std::integral_constant<int, N_>{});
+#define SCMP_SHAPE(T_, N_)                         \
+  if constexpr (FORWARD || N_ <= 2)               \
+    if (s.tpr == T_ && s.nb == N_) return f(std::integral_constant<int, T_>{}, std::integral_constant<int, N_>{});
   SCMP_SHAPE(32, 1) SCMP_SHAPE(32, 2) SCMP_SHAPE(64, 2) SCMP_SHAPE(128, 2) SCMP_SHAPE(256, 2) SCMP_SHAPE(512, 2)
   SCMP_SHAPE(512, 4)
 #undef SCMP_SHAPE
@@ -679,20 +676,20 @@ static int blocks_per_sm(K kern, int threads) {
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) == cudaSuccess && n > 0 ? n : 1;
 }
 static cudaError_t launch_forward(const Args& a, int dtype, bool vec, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
   with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     if (a.cols > kMaxForward) {
-      forward_long_kernel<T><<<(unsigned)a.rows, 1024, 0, st>>>(a);
+      e = launch_overlapped(forward_long_kernel<T>, (unsigned)a.rows, 1024, 0, st, 1, a);
       return;
     }
-    with_shape(shape_for(a.cols), [&](auto tpr, auto nb) {
+    with_shape<true>(shape_for(a.cols), [&](auto tpr, auto nb) {
       constexpr int TPR = decltype(tpr)::value, NB = decltype(nb)::value, TH = block_threads<TPR>();
-      // as many blocks as the SMs hold, each with its next row on the way
       const long long blocks = (a.rows + TH / TPR - 1) / (TH / TPR);
       auto go = [&](auto kern, int per_sm) {
-        const int grid = (int)(blocks < 148LL * per_sm ? blocks : 148LL * per_sm);
-        kern<<<grid, TH, 0, st>>>(a);
+        e = launch_overlapped(kern, (unsigned)(blocks < 148LL * per_sm ? blocks : 148LL * per_sm), TH, 0, st, 1, a);
       };
+      // as many blocks as the SMs hold, each with its next row on the way
       if (vec) {
         static const int per_sm = blocks_per_sm(forward_kernel<T, true, TPR, NB>, TH);
         go(forward_kernel<T, true, TPR, NB>, per_sm);
@@ -702,31 +699,29 @@ static cudaError_t launch_forward(const Args& a, int dtype, bool vec, cudaStream
       }
     });
   });
-  count_launch();
-  return cudaGetLastError();
+  return e;
 }
 
 static cudaError_t launch_backward(const Args& a, int dtype, bool vec, int blocks, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
   with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     auto go = [&](auto src8) {
       constexpr bool S8 = decltype(src8)::value;
       if (a.cols > kMaxBackward) {
-        backward_long_kernel<T, S8><<<(unsigned)a.rows, 1024, 0, st>>>(a);
-        if (a.part) {
-          weight_grad_long_kernel<T, S8><<<dim3(cdiv(a.cols, 256), blocks), 256, 0, st>>>(a);
-          count_launch();
-        }
+        e = launch_overlapped(backward_long_kernel<T, S8>, (unsigned)a.rows, 1024, 0, st, 1, a);
+        if (a.part && e == cudaSuccess)
+          e = launch_overlapped(weight_grad_long_kernel<T, S8>, dim3(cdiv(a.cols, 256), blocks), 256, 0, st, 1, a);
         return;
       }
-      with_shape(shape_for(a.cols), [&](auto tpr, auto nb) {
-        constexpr int TPR = decltype(tpr)::value, NB = decltype(nb)::value > 2 ? 2 : decltype(nb)::value, TH = block_threads<TPR>();
+      with_shape<false>(shape_for(a.cols), [&](auto tpr, auto nb) {
+        constexpr int TPR = decltype(tpr)::value, NB = decltype(nb)::value, TH = block_threads<TPR>();
+        constexpr int smem = Ring<T, S8, TPR, NB>::BYTES;
         if (vec) {
-          constexpr int smem = Ring<T, S8, TPR, NB>::BYTES;
-          cudaFuncSetAttribute(backward_kernel<T, S8, true, TPR, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-          backward_kernel<T, S8, true, TPR, NB><<<blocks, TH, smem, st>>>(a);
+          e = cudaFuncSetAttribute(backward_kernel<T, S8, true, TPR, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+          if (e == cudaSuccess) e = launch_overlapped(backward_kernel<T, S8, true, TPR, NB>, blocks, TH, smem, st, 1, a);
         } else {
-          backward_kernel<T, S8, false, TPR, NB><<<blocks, TH, 0, st>>>(a);
+          e = launch_overlapped(backward_kernel<T, S8, false, TPR, NB>, blocks, TH, 0, st, 1, a);
         }
       });
     };
@@ -735,8 +730,7 @@ static cudaError_t launch_backward(const Args& a, int dtype, bool vec, int block
     else
       go(std::false_type{});
   });
-  count_launch();
-  return cudaGetLastError();
+  return e;
 }
 
 static int check_shape(const char* who, int dtype, int wdtype, long long rows, int cols) {
@@ -749,14 +743,11 @@ static int check_shape(const char* who, int dtype, int wdtype, long long rows, i
 
 }  // namespace ln
 
-cudaError_t launch_column_sum(const float* part, int parts, int sets, int cols, int dtype, void* out0, void* out1,
-                                     cudaStream_t st) {
-  with_dtype(dtype, [&](auto* tag) {
+cudaError_t launch_column_sum(const float* part, int parts, int sets, int cols, int dtype, void* out0, void* out1, cudaStream_t st) {
+  return with_dtype(dtype, [&](auto* tag) {
     using W = std::remove_pointer_t<decltype(tag)>;
-    ln::column_sum_kernel<W><<<dim3(cdiv(cols, 32), sets), 1024, 0, st>>>(part, parts, sets, cols, (W*)out0, (W*)out1);
+    return launch_overlapped(ln::column_sum_kernel<W>, dim3(cdiv(cols, 32), sets), 1024, 0, st, 1, part, parts, sets, cols, (W*)out0, (W*)out1);
   });
-  count_launch();
-  return cudaGetLastError();
 }
 
 }  // namespace scmp

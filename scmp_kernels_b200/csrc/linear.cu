@@ -1,5 +1,6 @@
 // The exact linear layer's C entry points, and the pass over dy that its
 // gradients share.
+#include "launch.cuh"
 #include "linear.cuh"
 #include "status.cuh"
 
@@ -21,18 +22,20 @@ struct DpreArgs {
   float* part;  // (gridDim.y, cols), or null
 };
 template <class T>
-__device__ __forceinline__ void store_operand8(void* out, long long plane, long long at, const float (&d)[8]) {
+__device__ __forceinline__ void store_operand8(void* out, long long plane, long long at, const F2 (&d)[4]) {
   if constexpr (sizeof(T) == 2) {
     stg8((T*)out + at, d);
   } else {
     uint32_t w[3][4];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
       uint32_t lo[3], hi[3];
-      split3(d[i], lo);
-      split3(d[i + 1], hi);
+      f2_split(d[i], a, b);
+      split3(a, lo);
+      split3(b, hi);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) w[p][i >> 1] = lo[p] | (hi[p] << 16);
+      for (int p = 0; p < 3; ++p) w[p][i] = lo[p] | (hi[p] << 16);
     }
 #pragma unroll
     for (int p = 0; p < 3; ++p)
@@ -68,36 +71,77 @@ __device__ __forceinline__ void dpre_load(const DpreArgs& a, long long row, int 
     r.pre = ldg8((const T*)a.pre + row * a.ldp + c);
   }
 }
+// act'(code * 2^e) for every code and the exponents between which it is neither
+// linear in the value nor constant: an 8-bit checkpoint's derivative is a lookup,
+// a few instructions where evaluating it takes thirty. Exponent bytes
+// kTableFirst .. kTableFirst + kTableRows - 1 (2^-14 .. 2^3); the rest, and NaN, are
+// evaluated.
+constexpr int kTableFirst = 113, kTableRows = 18;
 template <int ACT>
-__device__ __forceinline__ void times_grad(float (&d)[8], const float (&p)[8]) {
+__device__ __forceinline__ void fill_table(float* table) {
+  for (int i = threadIdx.x; i < kTableRows * 256; i += 256)
+    table[i] = act_grad(ACT, fmul((float)(int8_t)(i & 255), act8_scale(kTableFirst + (i >> 8))));
+}
+__device__ __forceinline__ bool in_table(uint32_t ex) { return ex - kTableFirst < (uint32_t)kTableRows; }
+__device__ __forceinline__ void times_table(F2 (&d)[4], uint2 codes, uint32_t ex, const float* table) {
+  const float* row = table + (ex - kTableFirst) * 256;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) d[j] *= act_grad(ACT, p[j]);
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w = j < 2 ? codes.x : codes.y;
+    const int s = 16 * (j & 1);
+    d[j] = mul2(d[j], f2(row[(w >> s) & 255], row[(w >> (s + 8)) & 255]));
+  }
+}
+template <int ACT>
+__device__ __forceinline__ void times_grad(F2 (&d)[4], const F2 (&p)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) d[j] = mul2(d[j], act_grad2<ACT>(p[j]));
 }
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
-  __shared__ float s[8][256];
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) dpre_kernel(DpreArgs a) {
+  __shared__ float s[VEC ? (kTableRows > 8 ? kTableRows : 8) : 8][256];  // the table, and at the end the groups' sums
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
   const int c0 = blockIdx.x * 256;
+  const bool lookup = VEC && a.codes && a.act != SCMP_ACT_NONE;
+  if (lookup) {
+    switch (a.act) {
+      case SCMP_ACT_RELU: fill_table<SCMP_ACT_RELU>(s[0]); break;
+      case SCMP_ACT_GELU: fill_table<SCMP_ACT_GELU>(s[0]); break;
+      case SCMP_ACT_GELU_TANH: fill_table<SCMP_ACT_GELU_TANH>(s[0]); break;
+      default: fill_table<SCMP_ACT_SILU>(s[0]);
+    }
+    __syncthreads();
+  }
   float sum[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) sum[j] = 0.f;
   const long long step = (long long)gridDim.y * 8;
+  let_next_start();
+  prior_done();
   if (VEC) {
     const int c = c0 + lane * 8;
     long long row = (long long)blockIdx.y * 8 + group;
+    F2 acc[4] = {f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
     if (c < a.cols && row < a.rows) {
-      DpreRaw<T> next;
-      dpre_load<T>(a, row, c, next);
-      for (; row < a.rows; row += step) {  // the next row's loads run under this row's arithmetic
-        const DpreRaw<T> cur = next;
-        if (row + step < a.rows) dpre_load<T>(a, row + step, c, next);
-        float d[8], p[8];
+      // two rows' loads run under a row's arithmetic
+      DpreRaw<T> next[2];
+      dpre_load<T>(a, row, c, next[0]);
+      if (row + step < a.rows) dpre_load<T>(a, row + step, c, next[1]);
+      for (; row < a.rows; row += step) {
+        const DpreRaw<T> cur = next[0];
+        next[0] = next[1];
+        if (row + 2 * step < a.rows) dpre_load<T>(a, row + 2 * step, c, next[1]);
+        F2 d[4], p[4];
         unpack8(cur.dy, d);
-        if (a.act != SCMP_ACT_NONE) {
+        if (lookup && in_table(cur.ex)) {
+          times_table(d, cur.codes, cur.ex, s[0]);
+        } else if (a.act != SCMP_ACT_NONE) {
           if (a.codes) {
-            const float sc = act8_scale(cur.ex);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = act8_value(j < 4 ? cur.codes.x : cur.codes.y, j & 3, sc);
+            const F2 sc = f2(act8_scale(cur.ex));
+            p[0] = mul2(act8_pair(cur.codes.x, 0), sc);
+            p[1] = mul2(act8_pair(cur.codes.x, 1), sc);
+            p[2] = mul2(act8_pair(cur.codes.y, 0), sc);
+            p[3] = mul2(act8_pair(cur.codes.y, 1), sc);
           } else {
             unpack8(cur.pre, p);
           }
@@ -110,9 +154,11 @@ __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
         }
         if (a.dpre) store_operand8<T>(a.dpre, a.rows * a.ldo, row * a.ldo + c, d);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += d[j];
+        for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], d[j]);
       }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f2_split(acc[j], sum[2 * j], sum[2 * j + 1]);
   } else {
     for (long long row = (long long)blockIdx.y * 8 + group; row < a.rows; row += step) {
       const T* dy = (const T*)a.dy + row * a.ldy;
@@ -137,6 +183,7 @@ __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
     }
   }
   if (!a.part) return;
+  __syncthreads();  // the table is done with
 #pragma unroll
   for (int j = 0; j < 8; ++j) s[group][VEC ? lane * 8 + j : j * 32 + lane] = sum[j];
   __syncthreads();
@@ -148,23 +195,17 @@ __global__ void __launch_bounds__(256) dpre_kernel(DpreArgs a) {
 static int dpre_row_blocks(long long rows, int cols) {
   const int cb = cdiv(cols, 256);
   const long long want = (rows + 7) / 8;
-  const int most = cdiv(148 * 4, cb);
+  const int most = 148 * 4 / cb > 0 ? 148 * 4 / cb : 1;
   return (int)(want < most ? (want > 0 ? want : 1) : most);
 }
 static cudaError_t launch_dpre(const DpreArgs& a, int dtype, int row_blocks, cudaStream_t st) {
   const size_t es = dtype_size(dtype);
   const bool vec = a.cols % 8 == 0 && rows_aligned16(a.dy, a.ldy, es) &&
                    (a.act == SCMP_ACT_NONE || (a.codes ? (reinterpret_cast<uintptr_t>(a.codes) & 7) == 0 : rows_aligned16(a.pre, a.ldp, es)));
-  with_dtype(dtype, [&](auto* tag) {
+  return with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    const dim3 grid(cdiv(a.cols, 256), row_blocks);
-    if (vec)
-      dpre_kernel<T, true><<<grid, 256, 0, st>>>(a);
-    else
-      dpre_kernel<T, false><<<grid, 256, 0, st>>>(a);
+    return launch_overlapped(vec ? dpre_kernel<T, true> : dpre_kernel<T, false>, dim3(cdiv(a.cols, 256), row_blocks), 256, 0, st, 1, a);
   });
-  count_launch();
-  return cudaGetLastError();
 }
 
 struct Carve {
@@ -235,15 +276,12 @@ static BackwardPlan plan_backward(Carve& c, int dtype, long long rows, int d, in
   if (parts & 4) p.part = c.take<float>((size_t)p.row_blocks * m);
   return p;
 }
-// The operand of a (rows, cols) tensor, staged into `room` when it has to be.
-static cudaError_t operand(const void* p, long long ld, long long rows, int cols, int dtype, char* room, bool mn, Operand& o,
-                           cudaStream_t st) {
-  o = {p, cols, rows, ld, 1, mn};
-  if (!room) return cudaSuccess;
-  o.p = room;
-  o.ld = pitch_of(cols);
-  o.planes = dtype == SCMP_F32 ? 3 : 1;
-  return launch_restage(p, rows, cols, ld, dtype, room, st);
+// The operand of a (rows, cols) tensor; where it has to be staged, into `room`
+// by a job added to the launch.
+static Operand operand(const void* p, long long ld, long long rows, int cols, int dtype, char* room, bool mn, RestageArgs& jobs) {
+  if (!room) return {p, cols, rows, ld, 1, mn};
+  jobs.add(p, rows, cols, ld, room, dtype);
+  return {room, cols, rows, pitch_of(cols), dtype == SCMP_F32 ? 3 : 1, mn};
 }
 
 static int check_shape(const char* who, int dtype, long long rows, int d, int m, int act) {
@@ -291,9 +329,9 @@ int scmp_linear_forward(const void* x, long long ldx, const void* weight, long l
     SCMP_CUDA(lin::launch_rows(x, ldx, weight, ldw, (int)rows, d, m, e, dtype, st), "linear_forward");
     return SCMP_OK;
   }
-  lin::Operand a, b;
-  SCMP_CUDA(lin::operand(x, ldx, rows, d, dtype, w.x, false, a, st), "linear_forward: x");
-  SCMP_CUDA(lin::operand(weight, ldw, m, d, dtype, w.w, false, b, st), "linear_forward: weight");
+  lin::RestageArgs jobs{};
+  const lin::Operand a = lin::operand(x, ldx, rows, d, dtype, w.x, false, jobs), b = lin::operand(weight, ldw, m, d, dtype, w.w, false, jobs);
+  SCMP_CUDA(lin::launch_restage(jobs, dtype, st), "linear_forward: operands");
   SCMP_CUDA(lin::launch_tc(a, b, rows, m, d, e, dtype, (float*)w.partial, st), "linear_forward");
   return SCMP_OK;
 }
@@ -337,38 +375,38 @@ int scmp_linear_backward(const void* dy, long long lddy, const void* x, long lon
   lin::Carve c{(char*)workspace};
   const lin::BackwardPlan w = lin::plan_backward(c, dtype, rows, d, m, activation, x8, parts, unal);
   if (c.off && (!workspace || workspace_bytes < c.off)) return fail(SCMP_ERR_WORKSPACE, "linear_backward: workspace missing or too small");
-  lin::Operand g{dy, m, rows, lddy, 1, false};
+  lin::RestageArgs jobs{};
+  lin::Operand g{dy, m, rows, lddy, 1, false}, wt{}, xs{};
   if (act || dbias) {
     lin::DpreArgs a{dy, pre, pre_codes, pre_exps, rows, lddy, ldpre, m, activation, w.dpre, lin::pitch_of(m), w.part};
     SCMP_CUDA(lin::launch_dpre(a, dtype, w.row_blocks, st), "linear_backward: activation");
-    if (dbias)
-      SCMP_CUDA(launch_column_sum(w.part, w.row_blocks, 1, m, bias_dtype, dbias, nullptr, st), "linear_backward: bias");
     if (w.dpre) g = {w.dpre, m, rows, lin::pitch_of(m), dtype == SCMP_F32 ? 3 : 1, false};
   } else {
-    SCMP_CUDA(lin::operand(dy, lddy, rows, m, dtype, w.dpre, false, g, st), "linear_backward: dy");
+    g = lin::operand(dy, lddy, rows, m, dtype, w.dpre, false, jobs);
   }
-  if (dx) {
-    lin::Operand b;
-    SCMP_CUDA(lin::operand(weight, ldw, m, d, dtype, w.w, true, b, st), "linear_backward: weight");
-    lin::Epilogue e{};
-    e.out = dx;
-    e.ldo = d;
-    SCMP_CUDA(lin::launch_tc(g, b, rows, d, m, e, dtype, (float*)w.partial, st), "linear_backward: dx");
-  }
+  if (dx) wt = lin::operand(weight, ldw, m, d, dtype, w.w, true, jobs);
   if (dweight) {
-    lin::Operand b;
     if (x8) {
+      // a checkpoint's values are exact in 16 bits
       const int t = dtype == SCMP_F32 ? SCMP_BF16 : dtype;
       SCMP_CUDA(launch_act8_unpack(x_codes, x_exps, rows, d, w.x, lin::pitch_of(d), t, st), "linear_backward: unpack");
-      b = {w.x, d, rows, lin::pitch_of(d), 1, true};
+      xs = {w.x, d, rows, lin::pitch_of(d), 1, true};
     } else {
-      SCMP_CUDA(lin::operand(x, ldx, rows, d, dtype, w.x, true, b, st), "linear_backward: x");
+      xs = lin::operand(x, ldx, rows, d, dtype, w.x, true, jobs);
     }
+  }
+  if (dbias) jobs.add_sum(w.part, w.row_blocks, m, dbias, bias_dtype);
+  SCMP_CUDA(lin::launch_restage(jobs, dtype, st), "linear_backward: operands");
+  lin::Epilogue e{};
+  e.ldo = d;
+  if (dx) {
+    e.out = dx;
+    SCMP_CUDA(lin::launch_tc(g, wt, rows, d, m, e, dtype, (float*)w.partial, st), "linear_backward: dx");
+  }
+  if (dweight) {
     g.mn = true;
-    lin::Epilogue e{};
     e.out = dweight;
-    e.ldo = d;
-    SCMP_CUDA(lin::launch_tc(g, b, m, d, rows, e, dtype, (float*)w.partial, st), "linear_backward: dweight");
+    SCMP_CUDA(lin::launch_tc(g, xs, m, d, rows, e, dtype, (float*)w.partial, st), "linear_backward: dweight");
   }
   return SCMP_OK;
 }

@@ -86,6 +86,79 @@ __device__ __forceinline__ float act_grad(int act, float v) {
   }
 }
 
+// The same for two values at a time.
+__device__ __forceinline__ F2 reciprocal2(F2 x) {
+  float lo, hi;
+  f2_split(x, lo, hi);
+  return f2(reciprocal(lo), reciprocal(hi));
+}
+__device__ __forceinline__ F2 exp2_fast2(F2 x) {
+  float lo, hi;
+  f2_split(x, lo, hi);
+  return f2(exp2_fast(lo), exp2_fast(hi));
+}
+__device__ __forceinline__ F2 abs2(F2 x) { return {x.v & 0x7FFFFFFF7FFFFFFFull}; }
+__device__ __forceinline__ F2 min2(F2 x, float y) {
+  float lo, hi;
+  f2_split(x, lo, hi);
+  return f2(fminf(lo, y), fminf(hi, y));
+}
+// (The polynomial a value at a time: a coefficient is then part of the
+// instruction, where a pair would need it in two registers.)
+__device__ __forceinline__ F2 normal_tail2(F2 z, F2& e) {
+  float z0, z1, e0, e1;
+  f2_split(z, z0, z1);
+  const float q0 = normal_tail(z0, e0), q1 = normal_tail(z1, e1);
+  e = f2(e0, e1);
+  return f2(q0, q1);
+}
+// Phi(v) from Phi(-|v|)
+__device__ __forceinline__ F2 normal_cdf2(F2 v, F2 tail) {
+  float a, b, q0, q1, r0, r1;
+  f2_split(v, a, b);
+  f2_split(tail, q0, q1);
+  f2_split(fma2(tail, f2(-1.f), f2(1.f)), r0, r1);
+  return f2(a >= 0.f ? r0 : q0, b >= 0.f ? r1 : q1);
+}
+__device__ __forceinline__ F2 exp_minus2(F2 v) { return exp2_fast2(min2(mul2(v, f2(-1.4426950408889634f)), 115.f)); }
+__device__ __forceinline__ F2 sigmoid2(F2 v) { return reciprocal2(add2(f2(1.f), exp2_fast2(mul2(v, f2(-1.4426950408889634f))))); }
+__device__ __forceinline__ F2 gelu_tanh_arg2(F2 v) {
+  return mul2(f2(1.5957691216057308f), fma2(mul2(mul2(v, v), f2(0.044715f)), v, v));
+}
+template <int ACT>
+__device__ __forceinline__ F2 act_value2(F2 v) {
+  if constexpr (ACT == SCMP_ACT_GELU) {
+    F2 e;
+    return mul2(v, normal_cdf2(v, normal_tail2(abs2(v), e)));
+  } else if constexpr (ACT == SCMP_ACT_GELU_TANH) {
+    return mul2(v, sigmoid2(gelu_tanh_arg2(v)));
+  } else if constexpr (ACT == SCMP_ACT_SILU) {
+    return mul2(v, sigmoid2(v));
+  } else {
+    float lo, hi;
+    f2_split(v, lo, hi);
+    return f2(act_value(ACT, lo), act_value(ACT, hi));
+  }
+}
+template <int ACT>
+__device__ __forceinline__ F2 act_grad2(F2 v) {
+  if constexpr (ACT == SCMP_ACT_GELU) {
+    F2 e;
+    const F2 q = normal_tail2(abs2(v), e);
+    return fma2(mul2(v, f2(0.39894228040143268f)), e, normal_cdf2(v, q));
+  } else if constexpr (ACT == SCMP_ACT_GELU_TANH) {
+    const F2 e = exp_minus2(gelu_tanh_arg2(v)), s = reciprocal2(add2(f2(1.f), e));
+    return fma2(mul2(v, mul2(mul2(e, s), s)), mul2(f2(1.5957691216057308f), fma2(mul2(v, f2(0.134145f)), v, f2(1.f))), s);
+  } else if constexpr (ACT == SCMP_ACT_SILU) {
+    const F2 e = exp_minus2(v), s = reciprocal2(add2(f2(1.f), e));
+    return mul2(s, fma2(v, mul2(e, s), f2(1.f)));
+  } else {
+    float lo, hi;
+    f2_split(v, lo, hi);
+    return f2(act_grad(ACT, lo), act_grad(ACT, hi));
+  }
+}
+
 // What happens to an output element after the product's sum.
 struct Epilogue {
   const void* bias;      // (m) or null

@@ -10,6 +10,7 @@
 // nothing where memory is the bound). The order of a sum's terms is free, so
 // a lane's eight consecutive values serve as the fragment's k pairs as they
 // come. float32 multiplies on the CUDA cores.
+#include "launch.cuh"
 #include "linear.cuh"
 #include "status.cuh"
 
@@ -74,11 +75,13 @@ __device__ __forceinline__ void finish_element(const RowsArgs& a, float v, int r
 
 // NT: groups of eight rows of x. MT: groups of 16 weight rows. VEC: rows of x and w can be read 16 bytes at a time.
 template <class T, int NT, int MT, bool VEC>
-__global__ void __launch_bounds__(32 * ROWS_WARPS) rows_mma_kernel(RowsArgs a) {
+__global__ void __launch_bounds__(32 * ROWS_WARPS, !VEC ? 1 : NT == 1 ? 4 : NT == 2 ? 3 : 2) rows_mma_kernel(RowsArgs a) {
   __shared__ float part[ROWS_WARPS][NT * 8][MT * 16 + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int m0 = blockIdx.x * 16 * MT;
   const uint16_t* w0 = (const uint16_t*)a.w + (long long)(m0 + g) * a.ldw;
+  let_next_start();
+  prior_done();
   float acc[MT][NT][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -86,9 +89,10 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) rows_mma_kernel(RowsArgs a) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
-  // warps take turns of 32 * U columns
-  constexpr int U = 4;
-  for (int k0 = warp * 32 * U; k0 < a.d; k0 += ROWS_WARPS * 32 * U) {
+  // Warps take turns of 128 columns (whatever MT, so that a sum's order does not
+  // depend on it), 32 * U of them at a time: 128 bytes on the way per lane.
+  constexpr int U = MT == 2 ? 2 : 4;
+  for (int k0 = warp * 128; k0 < a.d; k0 += (k0 & 127) == 128 - 32 * U ? ROWS_WARPS * 128 - (128 - 32 * U) : 32 * U) {
     uint4 wq[MT][2][U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -141,6 +145,8 @@ __global__ void __launch_bounds__(512) rows_f32_kernel(RowsArgs a) {
   const float* w0 = (const float*)a.w + (long long)min(m0, a.m - 1) * a.ldw;
   const float* w1 = (const float*)a.w + (long long)min(m0 + 1, a.m - 1) * a.ldw;
   const float* x = (const float*)a.x;
+  let_next_start();
+  prior_done();
   float acc[2][NR];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -210,16 +216,14 @@ static bool few_rows(int dtype, long long rows) { return rows <= (dtype == SCMP_
 static cudaError_t launch_rows(const void* x, long long ldx, const void* w, long long ldw, int rows, int d, int m,
                                const Epilogue& e, int dtype, cudaStream_t st) {
   const RowsArgs a{x, w, ldx, ldw, rows, d, m, e};
+  cudaError_t err = cudaSuccess;
   const size_t es = dtype_size(dtype);
   const bool vec = rows_aligned16(x, ldx, es) && rows_aligned16(w, ldw, es) && (size_t)d * es % 16 == 0;
   if (dtype == SCMP_F32) {
     const int grid = cdiv(m, 32);
     auto go = [&](auto nr) {
       constexpr int NR = decltype(nr)::value;
-      if (vec)
-        rows_f32_kernel<NR, true><<<grid, 512, 0, st>>>(a);
-      else
-        rows_f32_kernel<NR, false><<<grid, 512, 0, st>>>(a);
+      err = launch_overlapped(vec ? rows_f32_kernel<NR, true> : rows_f32_kernel<NR, false>, grid, 512, 0, st, 1, a);
     };
     if (rows <= 1) go(std::integral_constant<int, 1>{});
     else if (rows <= 4) go(std::integral_constant<int, 4>{});
@@ -232,17 +236,10 @@ static cudaError_t launch_rows(const void* x, long long ldx, const void* w, long
     auto go = [&](auto* tag, auto nt) {
       using T = std::remove_pointer_t<decltype(tag)>;
       constexpr int NT = decltype(nt)::value;
-      if (mt == 2) {
-        if (vec)
-          rows_mma_kernel<T, NT, 2, true><<<grid, 32 * ROWS_WARPS, 0, st>>>(a);
-        else
-          rows_mma_kernel<T, NT, 2, false><<<grid, 32 * ROWS_WARPS, 0, st>>>(a);
-      } else {
-        if (vec)
-          rows_mma_kernel<T, NT, 1, true><<<grid, 32 * ROWS_WARPS, 0, st>>>(a);
-        else
-          rows_mma_kernel<T, NT, 1, false><<<grid, 32 * ROWS_WARPS, 0, st>>>(a);
-      }
+      if (mt == 2)
+        err = launch_overlapped(vec ? rows_mma_kernel<T, NT, 2, true> : rows_mma_kernel<T, NT, 2, false>, grid, 32 * ROWS_WARPS, 0, st, 1, a);
+      else
+        err = launch_overlapped(vec ? rows_mma_kernel<T, NT, 1, true> : rows_mma_kernel<T, NT, 1, false>, grid, 32 * ROWS_WARPS, 0, st, 1, a);
     };
     auto type = [&](auto* tag) {
       if (rows <= 8) go(tag, std::integral_constant<int, 1>{});
@@ -252,8 +249,7 @@ static cudaError_t launch_rows(const void* x, long long ldx, const void* w, long
     if (dtype == SCMP_BF16) type((__nv_bfloat16*)nullptr);
     else type((__half*)nullptr);
   }
-  count_launch();
-  return cudaGetLastError();
+  return err;
 }
 
 }  // namespace lin

@@ -30,6 +30,7 @@
 // SCMP_ERR_TIMEOUT and all roles leave.
 #include <cuda.h>
 
+#include "launch.cuh"
 #include "linear.cuh"
 #include "status.cuh"
 
@@ -42,14 +43,15 @@ constexpr int TC_THREADS = 128 + 32 * EPI_WARPS;
 constexpr int ACC_COLS = 256;     // tensor-memory columns between the two accumulators
 constexpr int MAX_SEGMENTS = 6;
 
-template <class T, int BN>
+template <class T, int BN, bool FULL>
 struct Cfg {
   static constexpr int A_BYTES = 128 * KB * 2;
   static constexpr int B_BYTES = BN / 2 * KB * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int PIECE = 32 * 32 * sizeof(T);          // a 32 x 32 piece of the result
-  static constexpr int STG = EPI_WARPS * 2 * PIECE;          // per epilogue warp: result and residual
-  static constexpr int STAGES = BN == 256 ? (sizeof(T) == 4 ? 5 : 6) : (sizeof(T) == 4 ? 6 : 8);
+  static constexpr int RES = FULL ? 2 : 0;                   // pieces of the residual on their way
+  static constexpr int STG = EPI_WARPS * (2 + RES) * PIECE;  // per epilogue warp: two pieces of the result as well
+  static constexpr int STAGES = (227 * 1024 - 1536 - STG) / STAGE;
   static constexpr int NP = BN / 64;            // 32-column pieces per epilogue warp
   static constexpr int SMEM = STAGES * STAGE + STG + 512 + 1024;
 };
@@ -65,6 +67,7 @@ struct TcArgs {
   int f16;               // operands are float16, else bfloat16
   int tma_out, tma_res, tma_pre;  // the tensor can be accessed by TMA (16-byte base and pitch)
   int vec_codes;                  // rows of codes can be written 16 bytes at a time
+  int vec_out, vec_pre;           // rows can be written four elements at a time
   float* partial;        // (tiles - whole, splits, 256, BN)
   Epilogue e;
 };
@@ -161,27 +164,31 @@ struct Piece {
   static __device__ __forceinline__ int slot(int row, int piece) {
     return row * PIECES + (piece ^ (PIECES == 4 ? (row >> 1) & 3 : row & 7));
   }
-  static __device__ __forceinline__ void put_row(uint4* s, int lane, const float (&v)[32]) {
+  static __device__ __forceinline__ void put_row(uint4* s, int lane, const F2 (&v)[16]) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      uint4 q;
       if constexpr (sizeof(T) == 2) {
         const T* t = nullptr;
-        q = make_uint4(pack2(v[8 * p], v[8 * p + 1], t), pack2(v[8 * p + 2], v[8 * p + 3], t), pack2(v[8 * p + 4], v[8 * p + 5], t),
-                       pack2(v[8 * p + 6], v[8 * p + 7], t));
+        s[slot(lane, p)] = make_uint4(pack_pair(v[4 * p], t), pack_pair(v[4 * p + 1], t), pack_pair(v[4 * p + 2], t), pack_pair(v[4 * p + 3], t));
       } else {
-        q = make_uint4(__float_as_uint(v[4 * p]), __float_as_uint(v[4 * p + 1]), __float_as_uint(v[4 * p + 2]), __float_as_uint(v[4 * p + 3]));
+        *reinterpret_cast<ulonglong2*>(s + slot(lane, p)) = make_ulonglong2(v[2 * p].v, v[2 * p + 1].v);
       }
-      s[slot(lane, p)] = q;
     }
   }
-  static __device__ __forceinline__ void add_row(const uint4* s, int lane, float (&v)[32]) {
+  static __device__ __forceinline__ void add_row(const uint4* s, int lane, F2 (&v)[16]) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const uint4 q = s[slot(lane, p)];
-      const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) v[p * PER + i] += Elem<T>::to_f(e[i]);
+      if constexpr (sizeof(T) == 2) {
+        const T* t = nullptr;
+        v[4 * p] = add2(v[4 * p], unpack_pair(q.x, t));
+        v[4 * p + 1] = add2(v[4 * p + 1], unpack_pair(q.y, t));
+        v[4 * p + 2] = add2(v[4 * p + 2], unpack_pair(q.z, t));
+        v[4 * p + 3] = add2(v[4 * p + 3], unpack_pair(q.w, t));
+      } else {
+        v[2 * p] = add2(v[2 * p], f2(__uint_as_float(q.x), __uint_as_float(q.y)));
+        v[2 * p + 1] = add2(v[2 * p + 1], f2(__uint_as_float(q.z), __uint_as_float(q.w)));
+      }
     }
   }
   // Tensors that TMA cannot access: a lane per column, row after row.
@@ -202,63 +209,75 @@ struct Piece {
 };
 
 template <int ACT>
-__device__ __forceinline__ void act_all(float (&v)[32]) {
+__device__ __forceinline__ void act_all(F2 (&v)[16]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] = act_value(ACT, v[j]);
+  for (int j = 0; j < 16; ++j) v[j] = act_value2<ACT>(v[j]);
 }
 
-// An epilogue warp's shared memory: a piece of the result, a piece of the
-// residual and the barrier of the residual's loads.
-struct WarpStage {
-  uint4* out;
-  uint4* res;
-  uint32_t bar;
-  uint32_t phase;
-};
-// Starts the load of a piece of the residual (one lane).
+// An epilogue warp's shared memory: two pieces of the result, and two of the
+// residual with their barriers.
 template <class T>
-__device__ __forceinline__ void start_residual(const Maps& maps, const WarpStage& w, long long row0, int col0) {
-  expect_tx(w.bar, Piece<T>::PIECES * 512);
-  tma_load_2d(smem_u32(w.res), &maps.res, col0, (int)row0, w.bar);
+struct WarpStage {
+  uint4* base;      // out 0, out 1, residual 0, residual 1
+  uint32_t bars;    // of residual 0 and 1
+  uint32_t phases;  // bit b: the phase residual b waits for
+  __device__ __forceinline__ uint4* out(int b) const { return base + b * (Piece<T>::PIECES * 32); }
+  __device__ __forceinline__ uint4* res(int b) const { return base + (2 + b) * (Piece<T>::PIECES * 32); }
+};
+// Starts the load of a piece of the residual into buffer b (one lane).
+template <class T>
+__device__ __forceinline__ void start_residual(const Maps& maps, const WarpStage<T>& w, int b, long long row0, int col0) {
+  expect_tx(w.bars + 8 * b, Piece<T>::PIECES * 512);
+  tma_load_2d(smem_u32(w.res(b)), &maps.res, col0, (int)row0, w.bars + 8 * b);
 }
 // Checkpoint, activation, residual and stores of a warp's 32 x 32 piece, a row
-// per lane in v (bias included). The residual's load is under way (TMA) and
-// replaced by that of next_col (if >= 0). False on a wait that gave up.
+// per lane in v (bias included), the p-th of its tile. The residual's load is
+// under way (TMA) and replaced by that of the piece after the next, at next_col
+// (if >= 0). False on a wait that gave up.
 template <class T, bool FULL>
-__device__ __forceinline__ bool finish_piece(const TcArgs& g, const Maps& maps, float (&v)[32], WarpStage& w, int lane, long long row0,
-                                             int col0, int next_col, volatile int* abort_flag) {
+__device__ __forceinline__ bool finish_piece(const TcArgs& g, const Maps& maps, F2 (&v)[16], WarpStage<T>& w, int lane, long long row0,
+                                             int col0, int p, int next_col, volatile int* abort_flag) {
   using P = Piece<T>;
   const Epilogue& e = g.e;
   const int rows = (int)(g.m - row0 < 32 ? g.m - row0 : 32);
-  if (lane == 0) tma_store_read();  // the piece before this one has left
+  uint4* out = w.out(p & 1);
+  if (lane == 0) {  // the piece that was in the buffer has left
+    if (FULL && e.pre)
+      tma_store_read();
+    else
+      asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+  }
   __syncwarp();
   if (FULL) {
     if (e.pre) {
-      P::put_row(w.out, lane, v);
+      P::put_row(out, lane, v);
       if (g.tma_pre) {
         fence_async();
         __syncwarp();
         if (lane == 0) {
-          tma_store(&maps.pre, smem_u32(w.out), col0, (int)row0);
+          tma_store(&maps.pre, smem_u32(out), col0, (int)row0);
           tma_store_read();
         }
       } else {
         __syncwarp();
-        P::store_rows(w.out, lane, (T*)e.pre, g.n, row0, rows, col0, g.n);
+        P::store_rows(out, lane, (T*)e.pre, g.n, row0, rows, col0, g.n);
       }
       __syncwarp();
     }
     if (e.codes) {
-      // the lane's 32 columns are one block of the checkpoint (columns past n count as zeros)
+      // The lane's 32 columns are one block of the checkpoint. Those past n are sums
+      // of zeros, or of a NaN or an infinity of the row, which its other columns show too.
       const int count = g.n - col0;
-      uint32_t top = 0;
+      float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) top = max(top, j < count ? __float_as_uint(v[j]) & 0x7FFFFFFFu : 0u);
-      const uint32_t byte = act8_exponent(top, act8_floor<T>());
-      const float inv = act8_inverse(byte);
+      for (int j = 0; j < 16; ++j) {
+        float a, b;
+        f2_split(v[j], a, b);
+        top = max_abs_nan(max_abs_nan(top, a), b);
+      }
+      const uint32_t byte = act8_exponent(__float_as_uint(top), act8_floor<T>());
       uint32_t c[8];
-#pragma unroll
-      for (int p = 0; p < 8; ++p) c[p] = act8_codes4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3], inv, byte == kAct8Nan);
+      act8_codes32(v, top, byte, c);
       if (lane < rows) {
         int8_t* dst = e.codes + (row0 + lane) * g.n + col0;
         if (g.vec_codes && count >= 32) {
@@ -280,26 +299,27 @@ __device__ __forceinline__ bool finish_piece(const TcArgs& g, const Maps& maps, 
       default: break;
     }
     if (e.residual) {
+      const int b = p & 1;
       if (g.tma_res) {
-        if (!mbar_wait(w.bar, w.phase & 1, abort_flag, 25)) return false;
-        ++w.phase;
+        if (!mbar_wait(w.bars + 8 * b, (w.phases >> b) & 1, abort_flag, 25)) return false;
+        w.phases ^= 1u << b;
       } else {
-        P::load_rows(w.res, lane, (const T*)e.residual, e.ldr, row0, rows, col0, g.n);
+        P::load_rows(w.res(b), lane, (const T*)e.residual, e.ldr, row0, rows, col0, g.n);
         __syncwarp();
       }
-      P::add_row(w.res, lane, v);
+      P::add_row(w.res(b), lane, v);
       __syncwarp();
-      if (g.tma_res && next_col >= 0 && lane == 0) start_residual<T>(maps, w, row0, next_col);
+      if (g.tma_res && next_col >= 0 && lane == 0) start_residual<T>(maps, w, b, row0, next_col);
     }
   }
-  P::put_row(w.out, lane, v);
+  P::put_row(out, lane, v);
   if (g.tma_out) {
     fence_async();
     __syncwarp();
-    if (lane == 0) tma_store(&maps.out, smem_u32(w.out), col0, (int)row0);
+    if (lane == 0) tma_store(&maps.out, smem_u32(out), col0, (int)row0);
   } else {
     __syncwarp();
-    P::store_rows(w.out, lane, (T*)e.out, e.ldo, row0, rows, col0, g.n);
+    P::store_rows(out, lane, (T*)e.out, e.ldo, row0, rows, col0, g.n);
     __syncwarp();
   }
   return true;
@@ -307,7 +327,7 @@ __device__ __forceinline__ bool finish_piece(const TcArgs& g, const Maps& maps, 
 // The bias of `pieces` times 32 columns into scratch (one float per column), and
 // from there the same values into every lane.
 template <class T, int NP>
-__device__ __forceinline__ void bias_rows(const TcArgs& g, float* scratch, int lane, int col0, float (&v)[NP][32]) {
+__device__ __forceinline__ void bias_rows(const TcArgs& g, float* scratch, int lane, int col0, F2 (&v)[NP][16]) {
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
     const int c = col0 + p * 32 + lane;
@@ -319,10 +339,8 @@ __device__ __forceinline__ void bias_rows(const TcArgs& g, float* scratch, int l
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const float4 b = reinterpret_cast<const float4*>(scratch)[p * 8 + q];
-      v[p][4 * q] = b.x;
-      v[p][4 * q + 1] = b.y;
-      v[p][4 * q + 2] = b.z;
-      v[p][4 * q + 3] = b.w;
+      v[p][2 * q] = f2(b.x, b.y);
+      v[p][2 * q + 1] = f2(b.z, b.w);
     }
   __syncwarp();
 }
@@ -330,15 +348,15 @@ __device__ __forceinline__ void bias_rows(const TcArgs& g, float* scratch, int l
 template <class T, bool A_MN, bool B_MN, int BN, bool FULL>
 __global__ void __launch_bounds__(TC_THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ TcArgs g) {
-  using C = Cfg<T, BN>;
+  using C = Cfg<T, BN, FULL>;
   constexpr int NST = C::STAGES;
   extern __shared__ char smem_raw[];
   char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(base);
   char* tail = base + NST * C::STAGE + C::STG;
   const uint32_t bars = smem_u32(tail);
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail + 8 * (2 * NST + 5 + EPI_WARPS));
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8 * (2 * NST + 5 + EPI_WARPS) + 4);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail + 8 * (2 * NST + 5 + 2 * EPI_WARPS));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8 * (2 * NST + 5 + 2 * EPI_WARPS) + 4);
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (NST + s); };
   auto accf = [&](int b) { return bars + 8u * (2 * NST + b); };
@@ -360,7 +378,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       mbar_init(acce(b), 2 * EPI_WARPS);
     }
     mbar_init(drain, 1);
-    for (int w = 0; w < EPI_WARPS; ++w) mbar_init(drain + 8 + 8 * w, 1);
+    for (int w = 0; w < 2 * EPI_WARPS; ++w) mbar_init(drain + 8 + 8 * w, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -378,6 +396,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   cluster_sync();
   tc_after();
   const uint32_t tmem = *tmem_slot;
+  let_next_start();
+  prior_done();
 
   constexpr bool PROMOTE = FULL || sizeof(T) == 4;
   const int tiles = g.tiles_m * g.tiles_n, items = g.whole + (tiles - g.whole) * g.splits;
@@ -496,8 +516,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     // registers: 384 threads x 168 at launch = 128 x 72 + 256 x 216
     if constexpr (PROMOTE) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int ew = warp - 4, quad = ew & 3, half = ew >> 2;
-    char* stg = base + NST * C::STAGE + ew * 2 * C::PIECE;
-    WarpStage ws{reinterpret_cast<uint4*>(stg), reinterpret_cast<uint4*>(stg + C::PIECE), drain + 8 + 8 * ew, 0};
+    char* stg = base + NST * C::STAGE + ew * (2 + C::RES) * C::PIECE;
+    WarpStage<T> ws{reinterpret_cast<uint4*>(stg), drain + 8 + 16 * ew, 0};
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     uint32_t n_acc = 0;
     bool ok = true;
@@ -507,31 +527,34 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const long long row0 = (long long)tm * 256 + rank * 128 + quad * 32;
       const int cols0 = tn * BN + half * (BN / 2);
       const bool live = row0 < g.m && cols0 < g.n;
-      if (FULL && g.e.residual && g.tma_res && live && part < 0 && lane == 0) start_residual<T>(maps, ws, row0, cols0);
+      if (FULL && g.e.residual && g.tma_res && live && part < 0 && lane == 0) {
+        start_residual<T>(maps, ws, 0, row0, cols0);
+        if (cols0 + 32 < g.n) start_residual<T>(maps, ws, 1, row0, cols0 + 32);
+      }
       // piece p of the tile, its sums in v
-      auto emit = [&](int p, float (&v)[32]) {
+      auto emit = [&](int p, F2 (&v)[16]) {
         const int col0 = cols0 + p * 32;
         if (row0 >= g.m || col0 >= g.n) return;
         if (part >= 0) {  // in the order in which join_kernel's lanes read it
-          float4* dst = reinterpret_cast<float4*>(g.partial) +
+          ulonglong2* dst = reinterpret_cast<ulonglong2*>(g.partial) +
                         ((((size_t)part * 2 + rank) * 4 + quad) * (BN / 32) + half * C::NP + p) * 256 + lane;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) dst[q * 32] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          for (int q = 0; q < 8; ++q) dst[q * 32] = make_ulonglong2(v[2 * q].v, v[2 * q + 1].v);
         } else {
-          ok = finish_piece<T, FULL>(g, maps, v, ws, lane, row0, col0, p + 1 < C::NP && col0 + 32 < g.n ? col0 + 32 : -1, abort_flag);
+          ok = finish_piece<T, FULL>(g, maps, v, ws, lane, row0, col0, p, p + 2 < C::NP && col0 + 64 < g.n ? col0 + 64 : -1, abort_flag);
         }
       };
       if constexpr (PROMOTE) {
-        float sum[C::NP][32];
+        F2 sum[C::NP][16];
         if (FULL && g.e.bias && part < 0) {
           if (lane == 0) tma_store_read();
           __syncwarp();
-          bias_rows<T>(g, reinterpret_cast<float*>(ws.out), lane, cols0, sum);
+          bias_rows<T>(g, reinterpret_cast<float*>(ws.out(0)), lane, cols0, sum);
         } else {
 #pragma unroll
           for (int p = 0; p < C::NP; ++p)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[p][j] = 0.f;
+            for (int j = 0; j < 16; ++j) sum[p][j] = f2(0.f);
         }
         for (int c0 = k0; c0 < k1; c0 += chunk, ++n_acc) {
           const int buf = n_acc & 1;
@@ -549,7 +572,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             tmem_wait();
             if (q + 1 < 2 * C::NP) tmem_ld16(src + (q + 1) * 16, r[(q + 1) & 1]);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sum[q >> 1][(q & 1) * 16 + j] += __uint_as_float(r[q & 1][j]);
+            for (int j = 0; j < 8; ++j)
+              sum[q >> 1][(q & 1) * 8 + j] = add2(sum[q >> 1][(q & 1) * 8 + j], f2(__uint_as_float(r[q & 1][2 * j]), __uint_as_float(r[q & 1][2 * j + 1])));
           }
           tc_before();  // the accumulator is read: the MMAs may overwrite it
           __syncwarp();
@@ -558,9 +582,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         // one copy of the epilogue's code, which would not fit the instruction cache four times
 #pragma unroll 1
         for (int p = 0; p < C::NP && ok; ++p) {
-          float v[32];
+          F2 v[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < 16; ++j) {
             v[j] = sum[0][j];
 #pragma unroll
             for (int i = 1; i < C::NP; ++i) v[j] = p == i ? sum[i][j] : v[j];
@@ -581,9 +605,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             __syncwarp();
             if (lane == 0) arrive_cluster(leader_addr(acce(buf)));
           }
-          float v[32];
+          F2 v[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          for (int j = 0; j < 16; ++j) v[j] = f2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
           emit(p, v);
         }
         ++n_acc;
@@ -604,49 +628,87 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Adds the partial tiles in order and runs the epilogue: a warp per 32 x 32 piece.
+// Adds the partial tiles in order and runs the epilogue: a warp per four rows of
+// a 32 x 32 piece, four columns per lane (eight lanes hold a row's 32 columns, one
+// block of an 8-bit checkpoint).
+template <class T>
+__device__ __forceinline__ void store_some(T* p, const float (&v)[4], int count, bool vec) {
+  if (vec && count >= 4) {
+    stg4(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < count) p[i] = Elem<T>::from_f(v[i]);
+  }
+}
 template <class T, bool FULL>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Maps maps, const __grid_constant__ TcArgs g, int bn) {
-  __shared__ __align__(1024) uint4 stg[4][2][Piece<T>::PIECES * 32];
-  __shared__ uint64_t bars[4];
-  __shared__ int abort_s;
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs g, int bn) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t = g.whole + blockIdx.y, band = t / (8 * g.tiles_n), r0 = t - band * 8 * g.tiles_n;
   const int h = min(8, g.tiles_m - band * 8), tn = r0 / h, tm = band * 8 + r0 - tn * h;
-  const int piece = blockIdx.x * 4 + warp, strip = piece / (bn / 32), cp = piece - strip * (bn / 32);
-  const long long row0 = (long long)tm * 256 + strip * 32;
-  const int col0 = tn * bn + cp * 32;
-  WarpStage ws{stg[warp][0], stg[warp][1], smem_u32(&bars[warp]), 0};
-  if (lane == 0) {
-    mbar_init(ws.bar, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (threadIdx.x == 0) abort_s = 0;
-  __syncthreads();
-  if (row0 >= g.m || col0 >= g.n) return;  // whole warps
-  if (FULL && g.e.residual && g.tma_res && lane == 0) start_residual<T>(maps, ws, row0, col0);
-  float v[1][32];
-  if (FULL && g.e.bias) {
-    bias_rows<T>(g, reinterpret_cast<float*>(ws.out), lane, col0, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[0][j] = 0.f;
-  }
+  const int piece = blockIdx.x, strip = piece / (bn / 32), cp = piece - strip * (bn / 32);
+  const int r = warp * 4 + (lane & 3), quad = lane >> 2;
+  const long long row = (long long)tm * 256 + strip * 32 + r;
+  const int col0 = tn * bn + cp * 32, col = col0 + quad * 4, count = g.n - col;
+  let_next_start();
+  prior_done();
+  if (row - (lane & 3) >= g.m || col0 >= g.n) return;  // whole warps
+  const bool live = row < g.m;
+  const Epilogue& e = g.e;
   const size_t part_size = (size_t)64 * bn;  // float4s of a partial tile
-  const float4* p = reinterpret_cast<const float4*>(g.partial) + (size_t)blockIdx.y * g.splits * part_size + (size_t)piece * 256 + lane;
-#pragma unroll 2
-  for (int s = 0; s < g.splits; ++s) {
+  const float4* p = reinterpret_cast<const float4*>(g.partial) + (size_t)blockIdx.y * g.splits * part_size + (size_t)piece * 256 + quad * 32 + r;
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
+  if (FULL && live) {
+    if (e.bias) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float4 f = __ldg(p + s * part_size + q * 32);
-      v[0][4 * q] += f.x;
-      v[0][4 * q + 1] += f.y;
-      v[0][4 * q + 2] += f.z;
-      v[0][4 * q + 3] += f.w;
+      for (int k = 0; k < 4; ++k)
+        if (k < count) bias[k] = e.bias_f32 ? __ldg((const float*)e.bias + col + k) : ldg1((const T*)e.bias + col + k);
+    }
+    if (e.residual) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < count) res[k] = ldg1((const T*)e.residual + row * e.ldr + col + k);
     }
   }
-  finish_piece<T, FULL>(g, maps, v[0], ws, lane, row0, col0, -1, &abort_s);
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (live) {
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s) {
+      const float4 f = __ldg(p + s * part_size);
+      v[0] += f.x;
+      v[1] += f.y;
+      v[2] += f.z;
+      v[3] += f.w;
+    }
+  }
+  if (FULL) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += bias[k];
+    if (e.pre && live) store_some((T*)e.pre + row * g.n + col, v, count, g.vec_pre);
+    if (e.codes) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = max(top, k < count ? __float_as_uint(v[k]) & 0x7FFFFFFFu : 0u);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      const uint32_t byte = act8_exponent(top, act8_floor<T>());
+      const uint32_t w = act8_codes4(v[0], v[1], v[2], v[3], act8_inverse(byte), byte == kAct8Nan);
+      if (live) {
+        int8_t* dst = e.codes + row * g.n + col;
+        if (g.vec_codes && count >= 4) {
+          *reinterpret_cast<uint32_t*>(dst) = w;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < count) dst[k] = (int8_t)(w >> (8 * k));
+        }
+        if (quad == 0) e.exps[row * act8_blocks(g.n) + (col0 >> 5)] = (uint8_t)byte;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = act_value(e.act, v[k]) + res[k];
+  }
+  if (live) store_some((T*)e.out + row * e.ldo + col, v, count, g.vec_out);
 }
 
 // ---------------------------------------------------------------------------
@@ -739,29 +801,13 @@ static int plane_pairs(int planes_a, int planes_b) { return planes_a == 1 ? plan
 template <class T, bool A_MN, bool B_MN, int BN, bool FULL>
 static cudaError_t launch_tc_t(const Maps& maps, const TcArgs& g, cudaStream_t st) {
   auto kern = gemm_tc_kernel<T, A_MN, B_MN, BN, FULL>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (Cfg<T, BN>::SMEM));
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (Cfg<T, BN, FULL>::SMEM));
   if (e != cudaSuccess) return e;
   const int rest = g.tiles_m * g.tiles_n - g.whole;
   const long long items = g.whole + (long long)rest * g.splits;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * (items < PAIRS ? items : PAIRS)), 1, 1);
-  cfg.blockDim = dim3(TC_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = (Cfg<T, BN>::SMEM);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, maps, g);
-  count_launch();
-  if (e == cudaSuccess && rest > 0) {
-    join_kernel<T, FULL><<<dim3(BN / 32 * 8 / 4, rest), 128, 0, st>>>(maps, g, BN);
-    count_launch();
-    e = cudaGetLastError();
-  }
+  e = launch_overlapped(kern, (unsigned)(2 * (items < PAIRS ? items : PAIRS)), TC_THREADS, (Cfg<T, BN, FULL>::SMEM), st, 2, maps, g);
+  if (e == cudaSuccess && rest > 0)
+    e = launch_overlapped(join_kernel<T, FULL>, dim3(BN / 32 * 8, rest), 256, 0, st, 1, g, BN);
   return e;
 }
 
@@ -794,6 +840,8 @@ static cudaError_t launch_tc(const Operand& a, const Operand& b, long long m, in
   g.tma_res = e.residual && rows_aligned16(e.residual, e.ldr, es);
   g.tma_pre = e.pre && rows_aligned16(e.pre, n, es);
   g.vec_codes = aligned16(e.codes) && n % 16 == 0;
+  g.vec_out = rows_aligned4(e.out, e.ldo, es);
+  g.vec_pre = rows_aligned4(e.pre, n, es);
   Maps maps;
   if (!make_map(&maps.a, a, g.f16, 128) || !make_map(&maps.b, b, g.f16, sc.bn / 2) ||
       (g.tma_out && !make_piece_map(&maps.out, e.out, m, n, e.ldo, dtype)) ||
@@ -814,18 +862,49 @@ static cudaError_t launch_tc(const Operand& a, const Operand& b, long long m, in
 // operands that TMA cannot read in place
 // ---------------------------------------------------------------------------
 // Rows at a 16-byte pitch; a float32 matrix as three bfloat16 planes (split3).
+// One launch does all of a call's, and the bias's gradient along with them.
+struct RestageJob {
+  const void* x;
+  long long rows, ld, ldo;
+  int cols;
+  bool vec;
+  FastDiv by;
+  void* out;
+};
+static long long pitch_of(int cols) { return (cols + 7) / 8 * 8LL; }
+struct RestageArgs {
+  RestageJob job[3];
+  int jobs;
+  long long most;     // items of the largest job
+  const float* part;  // column sums of the bias's gradient, or null
+  int parts, cols, sum_dtype;
+  void* sum;
+  void add(const void* x, long long rows, int cols_, long long ld, void* out, int dtype) {
+    job[jobs++] = {x, rows, ld, pitch_of(cols_), cols_, rows_aligned16(x, ld, dtype_size(dtype)), FastDiv(cdiv(cols_, 8)), out};
+    const long long items = rows * cdiv(cols_, 8);
+    if (items > most) most = items;
+  }
+  void add_sum(const float* part_, int parts_, int cols_, void* out, int dtype) {
+    part = part_;
+    parts = parts_;
+    cols = cols_;
+    sum = out;
+    sum_dtype = dtype;
+  }
+};
 template <class T>
-__global__ void __launch_bounds__(256) restage_kernel(const T* __restrict__ x, long long rows, int cols, long long ld,
-                                                      uint16_t* __restrict__ out, long long ldo, bool vec, FastDiv by) {
-  const int oct = cdiv(cols, 8);
-  const long long total = rows * oct, plane = rows * ldo;
+__device__ __forceinline__ void restage_one(const RestageJob& b) {
+  const T* x = (const T*)b.x;
+  uint16_t* out = (uint16_t*)b.out;
+  const int cols = b.cols;
+  const long long total = b.rows * b.by.d, plane = b.rows * b.ldo;
   for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
     long long row;
     int c;
-    row_and_piece(t, by, total < 1LL << 31, row, c);
+    row_and_piece(t, b.by, total < 1LL << 31, row, c);
     c *= 8;
-    const T* src = x + row * ld + c;
-    uint16_t* dst = out + row * ldo + c;
+    const T* src = x + row * b.ld + c;
+    uint16_t* dst = out + row * b.ldo + c;
     if constexpr (sizeof(T) == 2) {
       uint16_t v[8];
 #pragma unroll
@@ -833,7 +912,7 @@ __global__ void __launch_bounds__(256) restage_kernel(const T* __restrict__ x, l
       *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
     } else {
       float v[8];
-      if (vec && c + 8 <= cols) {
+      if (b.vec && c + 8 <= cols) {
         unpack8(ldg8(src), v);
       } else {
 #pragma unroll
@@ -853,16 +932,47 @@ __global__ void __launch_bounds__(256) restage_kernel(const T* __restrict__ x, l
     }
   }
 }
-static long long pitch_of(int cols) { return (cols + 7) / 8 * 8LL; }
-static cudaError_t launch_restage(const void* x, long long rows, int cols, long long ld, int dtype, void* out, cudaStream_t st) {
-  const long long items = rows * cdiv(cols, 8);
-  const int grid = (int)((items + 255) / 256 < 148 * 8 ? (items + 255) / 256 : 148 * 8);
-  if (dtype == SCMP_F32)
-    restage_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, cols, ld, (uint16_t*)out, pitch_of(cols), rows_aligned16(x, ld, 4), FastDiv(cdiv(cols, 8)));
-  else
-    restage_kernel<__half><<<grid, 256, 0, st>>>((const __half*)x, rows, cols, ld, (uint16_t*)out, pitch_of(cols), false, FastDiv(cdiv(cols, 8)));
-  count_launch();
-  return cudaGetLastError();
+template <class T>
+__global__ void __launch_bounds__(256) restage_kernel(const __grid_constant__ RestageArgs a) {
+  __shared__ float s[8][33];
+  let_next_start();
+  prior_done();
+  if ((int)blockIdx.y < a.jobs) {
+    restage_one<T>(a.job[blockIdx.y]);
+    return;
+  }
+  // column sums, 32 columns per block: eight strands of rows, each in order
+  const int lx = threadIdx.x & 31, ly = threadIdx.x >> 5;
+  for (int c0 = blockIdx.x * 32; c0 < a.cols; c0 += gridDim.x * 32) {
+    float v = 0.f;
+    if (c0 + lx < a.cols) {
+#pragma unroll 8
+      for (int p = ly; p < a.parts; p += 8) v += __ldg(a.part + (size_t)p * a.cols + c0 + lx);
+    }
+    __syncthreads();
+    s[ly][lx] = v;
+    __syncthreads();
+    if (ly == 0 && c0 + lx < a.cols) {
+#pragma unroll
+      for (int y = 1; y < 8; ++y) v += s[y][lx];
+      if (a.sum_dtype == SCMP_F32)
+        ((float*)a.sum)[c0 + lx] = v;
+      else
+        ((T*)a.sum)[c0 + lx] = Elem<T>::from_f(v);
+    }
+  }
+}
+static cudaError_t launch_restage(const RestageArgs& a, int dtype, cudaStream_t st) {
+  const int rows = a.jobs + (a.sum ? 1 : 0);
+  if (!rows) return cudaSuccess;
+  long long blocks = (a.most + 255) / 256;
+  const long long sums = a.sum ? cdiv(a.cols, 32) : 0;
+  if (blocks < sums) blocks = sums;
+  if (blocks > 148 * 8) blocks = 148 * 8;
+  return with_dtype(dtype, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    return launch_overlapped(restage_kernel<T>, dim3((unsigned)blocks, rows), 256, 0, st, 1, a);
+  });
 }
 
 }  // namespace lin
