@@ -98,7 +98,7 @@ __device__ __forceinline__ void times_grad(F2 (&d)[4], const F2 (&p)[4]) {
   for (int j = 0; j < 4; ++j) d[j] = mul2(d[j], act_grad2<ACT>(p[j]));
 }
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) dpre_kernel(DpreArgs a) {
+__global__ void __launch_bounds__(256, 3) dpre_kernel(DpreArgs a) {
   __shared__ float s[VEC ? (kTableRows > 8 ? kTableRows : 8) : 8][256];  // the table, and at the end the groups' sums
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
   const int c0 = blockIdx.x * 256;
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) dpre_kernel(DpreA
 static int dpre_row_blocks(long long rows, int cols) {
   const int cb = cdiv(cols, 256);
   const long long want = (rows + 7) / 8;
-  const int most = 148 * 4 / cb > 0 ? 148 * 4 / cb : 1;
+  const int most = 148 * 3 / cb > 0 ? 148 * 3 / cb : 1;  // one wave of blocks, three per SM
   return (int)(want < most ? (want > 0 ? want : 1) : most);
 }
 static cudaError_t launch_dpre(const DpreArgs& a, int dtype, int row_blocks, cudaStream_t st) {
@@ -237,7 +237,7 @@ struct ForwardPlan {
 };
 static ForwardPlan plan_forward(Carve& c, int dtype, long long rows, int d, int m, int unal) {
   ForwardPlan p{};
-  p.rows = few_rows(dtype, rows);
+  p.rows = few_rows(rows);
   if (p.rows) return p;
   const bool f32 = dtype == SCMP_F32;
   if (f32 || (unal & kUnalignedX)) p.x = c.take<char>(staged_bytes(dtype, rows, d));

@@ -8,8 +8,8 @@
 // 16-row operand and the tokens as the 8 columns (tcgen05 would need the
 // operands in shared memory first and a tile of at least 64 rows, and gains
 // nothing where memory is the bound). The order of a sum's terms is free, so
-// a lane's eight consecutive values serve as the fragment's k pairs as they
-// come. float32 multiplies on the CUDA cores.
+// a lane's consecutive values serve as the fragment's k pairs as they come.
+// float32 goes as bfloat16 parts; one row multiplies on the CUDA cores.
 #include "launch.cuh"
 #include "linear.cuh"
 #include "status.cuh"
@@ -135,10 +135,10 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS, !VEC ? 1 : NT == 1 ? 4 : NT =
   }
 }
 
-// float32: a warp takes two weight rows, lanes along the columns; a block 32.
-template <int NR, bool VEC>
-__global__ void __launch_bounds__(512) rows_f32_kernel(RowsArgs a) {
-  __shared__ float sums[NR][32];
+// float32, one row: a warp takes two weight rows, lanes along the columns; a block 32.
+template <bool VEC>
+__global__ void __launch_bounds__(512) row_f32_kernel(RowsArgs a) {
+  __shared__ float sums[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = blockIdx.x * 32 + warp * 2;
   // rows past the end repeat the last one and are not stored
@@ -147,71 +147,143 @@ __global__ void __launch_bounds__(512) rows_f32_kernel(RowsArgs a) {
   const float* x = (const float*)a.x;
   let_next_start();
   prior_done();
-  float acc[2][NR];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int r = 0; r < NR; ++r) acc[i][r] = 0.f;
+  float acc[2] = {0.f, 0.f};
   if (VEC) {
     constexpr int U = 4;
     for (int k0 = lane * 4; k0 < a.d; k0 += 128 * U) {
       float4 p[U], q[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int k = k0 + 128 * u;
         p[u] = q[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k < a.d) {
-          p[u] = __ldg(reinterpret_cast<const float4*>(w0 + k));
-          q[u] = __ldg(reinterpret_cast<const float4*>(w1 + k));
+        if (k0 + 128 * u < a.d) {
+          p[u] = __ldg(reinterpret_cast<const float4*>(w0 + k0 + 128 * u));
+          q[u] = __ldg(reinterpret_cast<const float4*>(w1 + k0 + 128 * u));
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int k = k0 + 128 * u;
         if (k >= a.d) break;
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          if (r < a.rows) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(x + r * a.ldx + k));
-            acc[0][r] = fmaf(p[u].x, v.x, fmaf(p[u].y, v.y, fmaf(p[u].z, v.z, fmaf(p[u].w, v.w, acc[0][r]))));
-            acc[1][r] = fmaf(q[u].x, v.x, fmaf(q[u].y, v.y, fmaf(q[u].z, v.z, fmaf(q[u].w, v.w, acc[1][r]))));
-          }
-        }
+        const float4 v = __ldg(reinterpret_cast<const float4*>(x + k));
+        acc[0] = fmaf(p[u].x, v.x, fmaf(p[u].y, v.y, fmaf(p[u].z, v.z, fmaf(p[u].w, v.w, acc[0]))));
+        acc[1] = fmaf(q[u].x, v.x, fmaf(q[u].y, v.y, fmaf(q[u].z, v.z, fmaf(q[u].w, v.w, acc[1]))));
       }
     }
   } else {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = lane; k < a.d; k += 32) {
-      const float p = __ldg(w0 + k), q = __ldg(w1 + k);
+      const float v = __ldg(x + k);
+      acc[0] = fmaf(__ldg(w0 + k), v, acc[0]);
+      acc[1] = fmaf(__ldg(w1 + k), v, acc[1]);
+    }
+  }
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        if (r < a.rows) {
-          const float v = __ldg(x + r * a.ldx + k);
-          acc[0][r] = fmaf(p, v, acc[0][r]);
-          acc[1][r] = fmaf(q, v, acc[1][r]);
-        }
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+    if (lane == 0) sums[warp * 2 + i] = acc[i];
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const int j = blockIdx.x * 32 + lane;
+    finish_element<float>(a, sums[lane], 0, j, j < a.m);
+  }
+}
+
+// Four float32 as two k pairs of each of their three bfloat16 parts (split3
+// without its care for infinities: they become NaN here, in their own row or
+// column of the result alike).
+__device__ __forceinline__ void split_pairs(const float4& v, uint32_t (&lo)[3], uint32_t (&hi)[3]) {
+  float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    lo[p] = __byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x7632);
+    hi[p] = __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x7632);
+    if (p < 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] -= __uint_as_float(__float_as_uint(f[i]) & 0xFFFF0000u);
+    }
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ float4 load_f32(const float* row, int c, int cols, bool live) {
+  float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (VEC) {
+    if (live && c < cols) q = __ldg(reinterpret_cast<const float4*>(row + c));
+  } else if (live) {
+    if (c < cols) q.x = __ldg(row + c);
+    if (c + 1 < cols) q.y = __ldg(row + c + 1);
+    if (c + 2 < cols) q.z = __ldg(row + c + 2);
+    if (c + 3 < cols) q.w = __ldg(row + c + 3);
+  }
+  return q;
+}
+// float32, a few rows: the six products of bfloat16 parts (as in the tensor-core
+// product of many rows), split in registers. A product of each size has its own
+// accumulator, so that small ones do not cost the large one roundings. Two groups
+// of eight warps take 16 weight rows each.
+template <int NT, bool VEC>
+__global__ void __launch_bounds__(64 * ROWS_WARPS) rows_mma_f32_kernel(RowsArgs a) {
+  __shared__ float part[ROWS_WARPS][NT * 8][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int kw = warp & (ROWS_WARPS - 1), half = warp / ROWS_WARPS;
+  const int m0 = blockIdx.x * 32 + half * 16;
+  const float* w0 = (const float*)a.w + (long long)(m0 + g) * a.ldw;
+  const float* w1 = w0 + 8 * a.ldw;
+  const bool live0 = m0 + g < a.m, live1 = m0 + g + 8 < a.m;
+  let_next_start();
+  prior_done();
+  float acc[3][NT][4];
+#pragma unroll
+  for (int s = 0; s < 3; ++s)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[s][n][i] = 0.f;
+  constexpr int U = NT == 4 ? 2 : 4;  // 16 columns each, in turns of 16 * U
+  for (int k0 = kw * 16 * U; k0 < a.d; k0 += ROWS_WARPS * 16 * U) {
+    float4 wa[U], wb[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      wa[u] = load_f32<VEC>(w0, k0 + u * 16 + t * 4, a.d, live0);
+      wb[u] = load_f32<VEC>(w1, k0 + u * 16 + t * 4, a.d, live1);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t a0[3], a1[3], b0[3], b1[3];  // rows g and g + 8, first and second pair
+      split_pairs(wa[u], a0, a1);
+      split_pairs(wb[u], b0, b1);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int r = n * 8 + g;
+        uint32_t x0[3], x1[3];
+        split_pairs(load_f32<VEC>((const float*)a.x + (long long)r * a.ldx, k0 + u * 16 + t * 4, a.d, r < a.rows), x0, x1);
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int q = 0; p + q < 3; ++q)  // part p of w times part q of x
+            mma_16816(acc[p + q][n], a0[p], b0[p], a1[p], b1[p], x0[q], x1[q], (const __nv_bfloat16*)nullptr);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      float v = acc[i][r];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) sums[r][warp * 2 + i] = v;
-    }
+    for (int i = 0; i < 4; ++i)
+      part[kw][n * 8 + 2 * t + (i & 1)][16 * half + g + 8 * (i >> 1)] = (acc[2][n][i] + acc[1][n][i]) + acc[0][n][i];
   __syncthreads();
-  if (warp < a.rows) {
+  for (int r = warp; r < a.rows; r += 2 * ROWS_WARPS) {
     const int j = blockIdx.x * 32 + lane;
-    finish_element<float>(a, sums[warp][lane], warp, j, j < a.m);
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < ROWS_WARPS; ++w) v += part[w][r][lane];
+    finish_element<float>(a, v, r, j, j < a.m);
   }
 }
 
-// Rows up to which the weight's bytes bound the product (16-bit: four 8-row
-// groups of mma.sync; float32: eight rows of multiply-adds).
-static bool few_rows(int dtype, long long rows) { return rows <= (dtype == SCMP_F32 ? 8 : 32); }
+// Rows up to which the weight's bytes bound the product: four 8-row groups of
+// mma.sync.
+static bool few_rows(long long rows) { return rows <= 32; }
 
 static cudaError_t launch_rows(const void* x, long long ldx, const void* w, long long ldw, int rows, int d, int m,
                                const Epilogue& e, int dtype, cudaStream_t st) {
@@ -221,13 +293,14 @@ static cudaError_t launch_rows(const void* x, long long ldx, const void* w, long
   const bool vec = rows_aligned16(x, ldx, es) && rows_aligned16(w, ldw, es) && (size_t)d * es % 16 == 0;
   if (dtype == SCMP_F32) {
     const int grid = cdiv(m, 32);
-    auto go = [&](auto nr) {
-      constexpr int NR = decltype(nr)::value;
-      err = launch_overlapped(vec ? rows_f32_kernel<NR, true> : rows_f32_kernel<NR, false>, grid, 512, 0, st, 1, a);
+    auto go = [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      err = launch_overlapped(vec ? rows_mma_f32_kernel<NT, true> : rows_mma_f32_kernel<NT, false>, grid, 64 * ROWS_WARPS, 0, st, 1, a);
     };
-    if (rows <= 1) go(std::integral_constant<int, 1>{});
-    else if (rows <= 4) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 8>{});
+    if (rows == 1) err = launch_overlapped(vec ? row_f32_kernel<true> : row_f32_kernel<false>, grid, 512, 0, st, 1, a);
+    else if (rows <= 8) go(std::integral_constant<int, 1>{});
+    else if (rows <= 16) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
   } else {
     // 32 weight rows per block halve x's reads; 16 fill the SMs with narrow layers (a
     // checkpoint's blocks need 32). An element's sum is the same either way.
