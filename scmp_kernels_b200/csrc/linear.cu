@@ -17,14 +17,24 @@ struct DpreArgs {
   const uint8_t* exps;
   long long rows, ldy, ldp;
   int cols, act;
-  void* dpre;   // rows at a pitch of ldo 16-bit values, float32 as three planes; or null
+  void* dpre;   // rows at a pitch of ldo 16-bit values, in `planes` planes; or null
+  int planes;   // float32: 3 (split3); 16-bit: 1, or 2 with the rounding's remainder
   long long ldo;
   float* part;  // (gridDim.y, cols), or null
 };
 template <class T>
-__device__ __forceinline__ void store_operand8(void* out, long long plane, long long at, const F2 (&d)[4]) {
+__device__ __forceinline__ void store_operand8(void* out, int planes, long long plane, long long at, const F2 (&d)[4]) {
   if constexpr (sizeof(T) == 2) {
     stg8((T*)out + at, d);
+    if (planes == 2) {
+      F2 rest[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T* t = nullptr;
+        rest[i] = fma2(unpack_pair(pack_pair(d[i], t), t), f2(-1.f), d[i]);
+      }
+      stg8((T*)out + plane + at, rest);
+    }
   } else {
     uint32_t w[3][4];
 #pragma unroll
@@ -43,9 +53,11 @@ __device__ __forceinline__ void store_operand8(void* out, long long plane, long 
   }
 }
 template <class T>
-__device__ __forceinline__ void store_operand1(void* out, long long plane, long long at, float v) {
+__device__ __forceinline__ void store_operand1(void* out, int planes, long long plane, long long at, float v) {
   if constexpr (sizeof(T) == 2) {
-    ((T*)out)[at] = Elem<T>::from_f(v);
+    const T r = Elem<T>::from_f(v);
+    ((T*)out)[at] = r;
+    if (planes == 2) ((T*)out)[plane + at] = Elem<T>::from_f(v - Elem<T>::to_f(r));
   } else {
     uint32_t p[3];
     split3(v, p);
@@ -152,7 +164,7 @@ __global__ void __launch_bounds__(256, 3) dpre_kernel(DpreArgs a) {
             default: times_grad<SCMP_ACT_SILU>(d, p);
           }
         }
-        if (a.dpre) store_operand8<T>(a.dpre, a.rows * a.ldo, row * a.ldo + c, d);
+        if (a.dpre) store_operand8<T>(a.dpre, a.planes, a.rows * a.ldo, row * a.ldo + c, d);
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] = add2(acc[j], d[j]);
       }
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(256, 3) dpre_kernel(DpreArgs a) {
         const int c = c0 + j * 32 + lane;
         if (c >= a.cols) continue;
         if (a.act != SCMP_ACT_NONE) v[j] *= act_grad(a.act, q[j]);
-        if (a.dpre) store_operand1<T>(a.dpre, a.rows * a.ldo, row * a.ldo + c, v[j]);
+        if (a.dpre) store_operand1<T>(a.dpre, a.planes, a.rows * a.ldo, row * a.ldo + c, v[j]);
         sum[j] += v[j];
       }
     }
@@ -220,8 +232,14 @@ struct Carve {
   }
 };
 // Bytes of a (rows, cols) operand staged for the product.
-static size_t staged_bytes(int dtype, long long rows, int cols) {
-  return (size_t)rows * pitch_of(cols) * 2 * (dtype == SCMP_F32 ? 3 : 1);
+static size_t staged_bytes(int planes, long long rows, int cols) { return (size_t)rows * pitch_of(cols) * 2 * planes; }
+static int planes_of(int dtype) { return dtype == SCMP_F32 ? 3 : 1; }
+// Planes of dpre. It is rounded to the 16-bit type for two products, each of
+// which rounds its result again; small products, whose time is launches, take the
+// remainder along as a second plane instead (a gigaflop, 2 us at most).
+static int dpre_planes(int dtype, long long rows, int d, int m, int act) {
+  if (dtype == SCMP_F32) return 3;
+  return act != SCMP_ACT_NONE && 2.0 * rows * d * m <= 2147483648.0 ? 2 : 1;
 }
 // Operands that are staged: float32 ones, and those TMA cannot read in place.
 constexpr int kUnalignedX = 1, kUnalignedWeight = 2, kUnalignedDy = 4;
@@ -240,8 +258,8 @@ static ForwardPlan plan_forward(Carve& c, int dtype, long long rows, int d, int 
   p.rows = few_rows(rows);
   if (p.rows) return p;
   const bool f32 = dtype == SCMP_F32;
-  if (f32 || (unal & kUnalignedX)) p.x = c.take<char>(staged_bytes(dtype, rows, d));
-  if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(dtype, m, d));
+  if (f32 || (unal & kUnalignedX)) p.x = c.take<char>(staged_bytes(planes_of(dtype), rows, d));
+  if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(planes_of(dtype), m, d));
   p.partial = c.take<char>(partial_bytes(rows, m, cdiv(d, KB), f32 ? 6 : 1));
   return p;
 }
@@ -251,25 +269,26 @@ struct BackwardPlan {
   char* w;      // weight staged
   char* partial;
   float* part;  // column sums of dpre per block row
-  int row_blocks;
+  int row_blocks, planes;
 };
 // parts: bit 0 dx, bit 1 dweight, bit 2 dbias
 static BackwardPlan plan_backward(Carve& c, int dtype, long long rows, int d, int m, int act, bool x8, int parts, int unal) {
   BackwardPlan p{};
   const bool f32 = dtype == SCMP_F32;
   p.row_blocks = dpre_row_blocks(rows, m);
-  if ((parts & 3) && (act != SCMP_ACT_NONE || f32 || (unal & kUnalignedDy))) p.dpre = c.take<char>(staged_bytes(dtype, rows, m));
+  p.planes = dpre_planes(dtype, rows, d, m, act);
+  if ((parts & 3) && (act != SCMP_ACT_NONE || f32 || (unal & kUnalignedDy))) p.dpre = c.take<char>(staged_bytes(p.planes, rows, m));
   size_t partial = 0;
   if (parts & 2) {
     if (x8)
-      p.x = c.take<char>(staged_bytes(SCMP_BF16, rows, d));
+      p.x = c.take<char>(staged_bytes(1, rows, d));
     else if (f32 || (unal & kUnalignedX))
-      p.x = c.take<char>(staged_bytes(dtype, rows, d));
-    partial = partial_bytes(m, d, (int)((rows + KB - 1) / KB), f32 ? (x8 ? 3 : 6) : 1);
+      p.x = c.take<char>(staged_bytes(planes_of(dtype), rows, d));
+    partial = partial_bytes(m, d, (int)((rows + KB - 1) / KB), plane_pairs(p.planes, f32 && !x8 ? 3 : 1));
   }
   if (parts & 1) {
-    if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(dtype, m, d));
-    const size_t q = partial_bytes(rows, d, cdiv(m, KB), f32 ? 6 : 1);
+    if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(planes_of(dtype), m, d));
+    const size_t q = partial_bytes(rows, d, cdiv(m, KB), plane_pairs(p.planes, f32 ? 3 : 1));
     if (q > partial) partial = q;
   }
   p.partial = c.take<char>(partial);
@@ -378,9 +397,9 @@ int scmp_linear_backward(const void* dy, long long lddy, const void* x, long lon
   lin::RestageArgs jobs{};
   lin::Operand g{dy, m, rows, lddy, 1, false}, wt{}, xs{};
   if (act || dbias) {
-    lin::DpreArgs a{dy, pre, pre_codes, pre_exps, rows, lddy, ldpre, m, activation, w.dpre, lin::pitch_of(m), w.part};
+    lin::DpreArgs a{dy, pre, pre_codes, pre_exps, rows, lddy, ldpre, m, activation, w.dpre, w.planes, lin::pitch_of(m), w.part};
     SCMP_CUDA(lin::launch_dpre(a, dtype, w.row_blocks, st), "linear_backward: activation");
-    if (w.dpre) g = {w.dpre, m, rows, lin::pitch_of(m), dtype == SCMP_F32 ? 3 : 1, false};
+    if (w.dpre) g = {w.dpre, m, rows, lin::pitch_of(m), w.planes, false};
   } else {
     g = lin::operand(dy, lddy, rows, m, dtype, w.dpre, false, jobs);
   }
