@@ -123,13 +123,16 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const int8_t* __restri
       for (int u = 0; u < U; ++u) {
         if (at[u] < 0) continue;
         const float s = act8_scale(ex[u]);
-        float v[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = act8_value(q[u][i >> 2], i & 3, s);
-        if constexpr (PER == 8)
+        if constexpr (PER == 8) {
+          const F2 s2 = f2(s), v[4] = {mul2(act8_pair(q[u][0], 0), s2), mul2(act8_pair(q[u][0], 1), s2), mul2(act8_pair(q[u][1], 0), s2),
+                                       mul2(act8_pair(q[u][1], 1), s2)};
           stg8(out + at[u], v);
-        else
+        } else {
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = act8_value(q[u][0], i, s);
           stg4(out + at[u], v);
+        }
       }
     }
   } else {
@@ -177,7 +180,7 @@ int scmp_act8_pack(const void* x, int dtype, long long rows, int cols, long long
   if (rows == 0) return SCMP_OK;
   if (!x || !codes || !exps) return fail(SCMP_ERR_INVALID_ARG, "act8_pack: null pointer");
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool vec = cols % 8 == 0 && rows_aligned16(x, ld, dtype_size(dtype)) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
+  const bool vec = cols % 8 == 0 && rows_aligned8(x, ld, dtype_size(dtype)) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
   const int grid = elementwise_grid(rows * act8_blocks(cols) * 4, vec ? 256 : 32);
   const cudaError_t e = with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;

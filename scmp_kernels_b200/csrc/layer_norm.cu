@@ -35,7 +35,7 @@ struct Args {
   const void* weight;  // may be null (ones)
   const void* bias;    // may be null (zeros)
   int w_f32;           // weight and bias are float32, not x's type
-  int w_vec;           // weight and bias are 16-byte aligned
+  int w_vec;           // weight and bias are 32-byte aligned
   void* out;
   float* mean;
   float* rstd;
@@ -767,10 +767,10 @@ int scmp_layer_norm_forward(const void* x, int dtype, long long rows, int cols, 
   ln::Args a{};
   a.rows = rows; a.cols = cols; a.ldx = ldx; a.ldo = cols; a.eps = eps;
   a.x = x; a.weight = weight; a.bias = bias; a.w_f32 = wdtype == SCMP_F32;
-  a.w_vec = aligned16(weight) && aligned16(bias);
+  a.w_vec = rows_aligned8(weight, 8, 4) && rows_aligned8(bias, 8, 4);
   a.out = y; a.mean = mean; a.rstd = rstd; a.codes_out = codes; a.exps_out = exps;
   const size_t es = dtype_size(dtype);
-  const bool vec = cols % 8 == 0 && rows_aligned16(x, ldx, es) && aligned16(y) &&
+  const bool vec = cols % 8 == 0 && rows_aligned8(x, ldx, es) && rows_aligned8(y, cols, es) &&
                    (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
   SCMP_CUDA(ln::launch_forward(a, dtype, vec, (cudaStream_t)stream), "layer_norm_forward");
   return SCMP_OK;
@@ -805,12 +805,12 @@ int scmp_layer_norm_backward(const void* dy, long long lddy, const void* x, long
   ln::Args a{};
   a.rows = rows; a.cols = cols; a.ldx = ldx; a.ldy = lddy; a.ldo = cols;
   a.x = x; a.codes = codes; a.exps = exps; a.dy = dy; a.weight = weight; a.w_f32 = wdtype == SCMP_F32;
-  a.w_vec = aligned16(weight);
+  a.w_vec = rows_aligned8(weight, 8, 4);
   a.out = dx; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.part = sums ? (float*)workspace : nullptr;
   const size_t es = dtype_size(dtype);
-  const bool vec = cols % 8 == 0 && rows_aligned16(dy, lddy, es) && aligned16(dx) &&
-                   (x ? rows_aligned16(x, ldx, es) : (reinterpret_cast<uintptr_t>(codes) & 7) == 0);
+  const bool vec = cols % 8 == 0 && rows_aligned8(dy, lddy, es) && rows_aligned8(dx, cols, es) &&
+                   (x ? rows_aligned8(x, ldx, es) : (reinterpret_cast<uintptr_t>(codes) & 7) == 0);
   SCMP_CUDA(ln::launch_backward(a, dtype, vec, blocks, st), "layer_norm_backward");
   if (sums)
     SCMP_CUDA(launch_column_sum(a.part, blocks, 2, cols, wdtype, dweight, dbias, st), "layer_norm_backward: column sums");

@@ -212,8 +212,8 @@ static int dpre_row_blocks(long long rows, int cols) {
 }
 static cudaError_t launch_dpre(const DpreArgs& a, int dtype, int row_blocks, cudaStream_t st) {
   const size_t es = dtype_size(dtype);
-  const bool vec = a.cols % 8 == 0 && rows_aligned16(a.dy, a.ldy, es) &&
-                   (a.act == SCMP_ACT_NONE || (a.codes ? (reinterpret_cast<uintptr_t>(a.codes) & 7) == 0 : rows_aligned16(a.pre, a.ldp, es)));
+  const bool vec = a.cols % 8 == 0 && rows_aligned8(a.dy, a.ldy, es) &&
+                   (a.act == SCMP_ACT_NONE || (a.codes ? (reinterpret_cast<uintptr_t>(a.codes) & 7) == 0 : rows_aligned8(a.pre, a.ldp, es)));
   return with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     return launch_overlapped(vec ? dpre_kernel<T, true> : dpre_kernel<T, false>, dim3(cdiv(a.cols, 256), row_blocks), 256, 0, st, 1, a);

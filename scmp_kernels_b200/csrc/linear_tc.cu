@@ -880,7 +880,7 @@ struct RestageArgs {
   int parts, cols, sum_dtype;
   void* sum;
   void add(const void* x, long long rows, int cols_, long long ld, void* out, int dtype) {
-    job[jobs++] = {x, rows, ld, pitch_of(cols_), cols_, rows_aligned16(x, ld, dtype_size(dtype)), FastDiv(cdiv(cols_, 8)), out};
+    job[jobs++] = {x, rows, ld, pitch_of(cols_), cols_, rows_aligned8(x, ld, dtype_size(dtype)), FastDiv(cdiv(cols_, 8)), out};
     const long long items = rows * cdiv(cols_, 8);
     if (items > most) most = items;
   }

@@ -60,17 +60,29 @@ __device__ __forceinline__ float ldg1(const T* p) {
   return Elem<T>::to_f(ldg_raw(p));
 }
 
-// Eight consecutive values as they lie in memory (16 or 32 bytes, 16-byte aligned).
+// Eight consecutive values as they lie in memory (16 or 32 bytes, aligned to
+// that), in one access: two of 16 bytes would each touch half of every 32-byte
+// sector of a warp's float32 row.
 template <class T>
 struct Raw8 {
   uint4 q[sizeof(T) * 8 / 16];
 };
+__device__ __forceinline__ void stg256(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x),
+               "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
 template <class T>
 __device__ __forceinline__ Raw8<T> ldg8(const T* p) {
   Raw8<T> r;
-  const uint4* s = reinterpret_cast<const uint4*>(p);
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(T) * 8 / 16); ++i) r.q[i] = __ldg(s + i);
+  if constexpr (sizeof(T) == 2) {
+    r.q[0] = __ldg(reinterpret_cast<const uint4*>(p));
+  } else {
+    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r.q[0].x), "=r"(r.q[0].y), "=r"(r.q[0].z), "=r"(r.q[0].w), "=r"(r.q[1].x), "=r"(r.q[1].y), "=r"(r.q[1].z),
+                   "=r"(r.q[1].w)
+                 : "l"(p));
+  }
   return r;
 }
 template <class T>
@@ -88,21 +100,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
   const __half2 p = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&p);
 }
-template <class T>
-__device__ __forceinline__ void stg8(T* p, const float (&v)[8]) {
-  Raw8<T> r;
-  if constexpr (sizeof(T) == 2) {
-    r.q[0] = make_uint4(pack2(v[0], v[1], p), pack2(v[2], v[3], p), pack2(v[4], v[5], p), pack2(v[6], v[7], p));
-  } else {
-    T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = v[i];
-  }
-  uint4* d = reinterpret_cast<uint4*>(p);
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(T) * 8 / 16); ++i) d[i] = r.q[i];
-}
-
 // Four consecutive values as they lie in memory (8 or 16 bytes, aligned to that).
 template <class T>
 struct Raw4 {
@@ -196,9 +193,8 @@ __device__ __forceinline__ void stg8(T* p, const F2 (&v)[4]) {
     const T* t = nullptr;
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_pair(v[0], t), pack_pair(v[1], t), pack_pair(v[2], t), pack_pair(v[3], t));
   } else {
-    ulonglong2* d = reinterpret_cast<ulonglong2*>(p);
-    d[0] = make_ulonglong2(v[0].v, v[1].v);
-    d[1] = make_ulonglong2(v[2].v, v[3].v);
+    const uint4* q = reinterpret_cast<const uint4*>(&v);
+    stg256(p, q[0], q[1]);
   }
 }
 
@@ -228,7 +224,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline bool rows_aligned4(const void* p, long long ld, size_t esize) {
   return reinterpret_cast<uintptr_t>(p) % (4 * esize) == 0 && ld % 4 == 0;
 }
-// Rows of `cols` elements at a pitch of ld elements can be read 16 bytes at a time.
+// Rows at a pitch of ld elements can be accessed eight elements at a time.
+inline bool rows_aligned8(const void* p, long long ld, size_t esize) {
+  return reinterpret_cast<uintptr_t>(p) % (8 * esize) == 0 && ld % 8 == 0;
+}
+// Rows at a pitch of ld elements start on multiples of 16 bytes.
 inline bool rows_aligned16(const void* p, long long ld, size_t esize) {
   return aligned16(p) && (size_t)ld * esize % 16 == 0;
 }
