@@ -13,6 +13,13 @@
 // all rows of its block, and leaves one partial row per block that a second
 // kernel adds in a fixed order: no atomics, the same bits every time. Rows too
 // long for registers take the three-pass kernels at the end.
+//
+// Measured (B200): forward 12608 x 768 float32 16.3 us (77 MB, 4.8 TB/s; the SMs'
+// last rows and the start are a fifth of it); backward 8192 x 8192 bfloat16 from an
+// 8-bit checkpoint 84 us (338 MB, 4.0 TB/s), 9 us of it the column sums: a row takes
+// an SM 1.4 us, half of them instructions (18 a value), half the row's two sums,
+// which a second row per SM (64 registers, or values taken twice: 119 to 152
+// us) did not hide.
 #include "act8.cuh"
 #include "launch.cuh"
 #include "status.cuh"

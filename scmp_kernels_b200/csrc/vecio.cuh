@@ -5,8 +5,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <type_traits>
-
 #include "common.cuh"
 
 namespace scmp {
@@ -100,22 +98,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
   const __half2 p = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&p);
 }
-// Four consecutive values as they lie in memory (8 or 16 bytes, aligned to that).
-template <class T>
-struct Raw4 {
-  using U = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
-  U q;
-};
-template <class T>
-__device__ __forceinline__ Raw4<T> ldg4(const T* p) {
-  return {__ldg(reinterpret_cast<const typename Raw4<T>::U*>(p))};
-}
-template <class T>
-__device__ __forceinline__ void unpack4(const Raw4<T>& r, float (&v)[4]) {
-  const T* e = reinterpret_cast<const T*>(&r);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = Elem<T>::to_f(e[i]);
-}
+// Four consecutive values (8 or 16 bytes, aligned to that).
 template <class T>
 __device__ __forceinline__ void stg4(T* p, const float (&v)[4]) {
   if constexpr (sizeof(T) == 2)

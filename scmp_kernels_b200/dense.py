@@ -15,6 +15,7 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _layers as L
 from . import _lib
@@ -59,8 +60,8 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Act8, None], weight
     their :class:`Act8`. x may be None with ``need_dweight=False``, weight with
     ``need_dx=False``; what is not asked for is None. dbias has ``bias_dtype``
     (default: dy's; or float32). The gradient of the pre-activation that the two
-    products share is rounded to dy's dtype once; dbias is summed before that
-    rounding.
+    products share is rounded to dy's dtype once (small layers keep the rest of it
+    as well); dbias is summed before that rounding.
     """
     act = _activation("linear_backward", activation)
     x8 = p8 = xe = pe = None
@@ -100,6 +101,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         weight, x, xe, pre, pe = ctx.saved_tensors
         x = Act8(x, xe, ctx.dtype) if xe is not None else x

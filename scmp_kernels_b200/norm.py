@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _layers as L
 from .act8 import Act8, _wrap
@@ -55,6 +56,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, exps, mean, rstd, weight = ctx.saved_tensors
         if exps is not None:
