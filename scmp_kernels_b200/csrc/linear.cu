@@ -262,7 +262,8 @@ static ForwardPlan plan_forward(Carve& c, int dtype, long long rows, int d, int 
   const bool f32 = dtype == SCMP_F32;
   if (f32 || (unal & kUnalignedX)) p.x = c.take<char>(staged_bytes(planes_of(dtype), rows, d));
   if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(planes_of(dtype), m, d));
-  p.partial = c.take<char>(partial_bytes(rows, m, cdiv(d, KB), f32 ? 6 : 1));
+  const Size size{rows, m, cdiv(d, KB), f32 ? 6 : 1};
+  p.partial = c.take<char>(partial_bytes(&size, 1));
   return p;
 }
 struct BackwardPlan {
@@ -280,20 +281,20 @@ static BackwardPlan plan_backward(Carve& c, int dtype, long long rows, int d, in
   p.row_blocks = dpre_row_blocks(rows, m);
   p.planes = dpre_planes(dtype, rows, d, m, act);
   if ((parts & 3) && (act != SCMP_ACT_NONE || f32 || (unal & kUnalignedDy))) p.dpre = c.take<char>(staged_bytes(p.planes, rows, m));
-  size_t partial = 0;
+  Size sizes[2];
+  int count = 0;
+  if (parts & 1) {
+    if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(planes_of(dtype), m, d));
+    sizes[count++] = {rows, d, cdiv(m, KB), plane_pairs(p.planes, f32 ? 3 : 1)};
+  }
   if (parts & 2) {
     if (x8)
       p.x = c.take<char>(staged_bytes(1, rows, d));
     else if (f32 || (unal & kUnalignedX))
       p.x = c.take<char>(staged_bytes(planes_of(dtype), rows, d));
-    partial = partial_bytes(m, d, (int)((rows + KB - 1) / KB), plane_pairs(p.planes, f32 && !x8 ? 3 : 1));
+    sizes[count++] = {m, d, (int)((rows + KB - 1) / KB), plane_pairs(p.planes, f32 && !x8 ? 3 : 1)};
   }
-  if (parts & 1) {
-    if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(planes_of(dtype), m, d));
-    const size_t q = partial_bytes(rows, d, cdiv(m, KB), plane_pairs(p.planes, f32 ? 3 : 1));
-    if (q > partial) partial = q;
-  }
-  p.partial = c.take<char>(partial);
+  if (count) p.partial = c.take<char>(partial_bytes(sizes, count));
   if (parts & 4) p.part = c.take<float>((size_t)p.row_blocks * m);
   return p;
 }
@@ -353,7 +354,8 @@ int scmp_linear_forward(const void* x, long long ldx, const void* weight, long l
   lin::RestageArgs jobs{};
   const lin::Operand a = lin::operand(x, ldx, rows, d, dtype, w.x, false, jobs), b = lin::operand(weight, ldw, m, d, dtype, w.w, false, jobs);
   SCMP_CUDA(lin::launch_restage(jobs, dtype, st), "linear_forward: operands");
-  SCMP_CUDA(lin::launch_tc(a, b, rows, m, d, e, dtype, (float*)w.partial, st), "linear_forward");
+  const lin::Product p{a, b, rows, d, m, e};
+  SCMP_CUDA(lin::launch_tc<lin::Kind::forward>(&p, dtype, (float*)w.partial, st), "linear_forward");
   return SCMP_OK;
 }
 
@@ -418,17 +420,14 @@ int scmp_linear_backward(const void* dy, long long lddy, const void* x, long lon
   }
   if (dbias) jobs.add_sum(w.part, w.row_blocks, m, dbias, bias_dtype);
   SCMP_CUDA(lin::launch_restage(jobs, dtype, st), "linear_backward: operands");
-  lin::Epilogue e{};
-  e.ldo = d;
-  if (dx) {
-    e.out = dx;
-    SCMP_CUDA(lin::launch_tc(g, wt, rows, d, m, e, dtype, (float*)w.partial, st), "linear_backward: dx");
-  }
-  if (dweight) {
-    g.mn = true;
-    e.out = dweight;
-    SCMP_CUDA(lin::launch_tc(g, xs, m, d, rows, e, dtype, (float*)w.partial, st), "linear_backward: dweight");
-  }
+  lin::Epilogue ex{}, ew{};
+  ex.ldo = ew.ldo = d;
+  ex.out = dx;
+  ew.out = dweight;
+  lin::Operand gt = g;
+  gt.mn = true;
+  const lin::Product px{g, wt, rows, m, d, ex}, pw{gt, xs, m, rows, d, ew};
+  SCMP_CUDA(lin::launch_gradients(dx ? &px : nullptr, dweight ? &pw : nullptr, dtype, (float*)w.partial, st), "linear_backward: products");
   return SCMP_OK;
 }
 

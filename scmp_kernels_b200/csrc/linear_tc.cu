@@ -26,7 +26,8 @@
 //
 // The last wave, when its tiles do not fill the SMs: their k blocks are split
 // over several clusters, which leave float32 partial tiles that a second kernel
-// adds in order and runs the epilogue on.
+// adds in order and runs the epilogue on. Small products are split over all SMs
+// that way, the two gradients of a small layer in one launch between them.
 //
 // Measured (B200, back to back): 4096 x 4096 x 8192 bfloat16 180 us, 1.53
 // PFLOP/s or 0.93 of the measured cuBLAS rate (alone, at full clock, 152 to 176
@@ -40,6 +41,8 @@
 // Every wait is bounded (common.cuh): on a timeout the kernel records
 // SCMP_ERR_TIMEOUT and all roles leave.
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "launch.cuh"
 #include "linear.cuh"
@@ -67,7 +70,16 @@ struct Cfg {
   static constexpr int SMEM = STAGES * STAGE + STG + 512 + 1024;
 };
 
-struct TcArgs {
+// What a launch computes. The forward pass's product has k-contiguous operands and
+// the whole epilogue; the gradients' have none of it: dx = dpre W reads W along its
+// tile axis, dweight = dpre^T x reads both operands along theirs, and `gradients`
+// is both, dx first, in one launch whose waves their tiles share.
+enum class Kind { forward, dx, dweight, gradients };
+template <Kind K>
+constexpr int kProducts = K == Kind::gradients ? 2 : 1;
+
+// One product.
+struct Problem {
   int m, n;              // output rows and columns
   int kblocks;           // k blocks of one plane pair
   int segments;          // plane pairs
@@ -75,12 +87,16 @@ struct TcArgs {
   int chunk;             // k blocks per accumulator chain (PROMOTE), of every plane pair
   int tiles_m, tiles_n;
   int whole, splits;     // tiles run whole; the others in `splits` parts each
-  int f16;               // operands are float16, else bfloat16
   int tma_out, tma_res, tma_pre;  // the tensor can be accessed by TMA (16-byte base and pitch)
   int vec_codes;                  // rows of codes can be written 16 bytes at a time
   int vec_out, vec_pre;           // rows can be written four elements at a time
   float* partial;        // (tiles - whole, splits, 256, BN)
   Epilogue e;
+};
+template <int N>
+struct TcArgs {
+  Problem p[N];
+  int f16;  // operands are float16, else bfloat16
 };
 
 __device__ __forceinline__ uint64_t desc_base(uint32_t lbo_bytes) {
@@ -151,6 +167,10 @@ __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.syn
 struct Maps {
   CUtensorMap a, b, out, pre, res;
 };
+template <int N>
+struct MapSet {
+  Maps p[N];
+};
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src)
                : "memory");
@@ -202,19 +222,47 @@ struct Piece {
       }
     }
   }
-  // Tensors that TMA cannot access: a lane per column, row after row.
+  // Tensors that TMA cannot access: V neighbouring columns per lane, V rows at a
+  // time; V is what their base and pitch are multiples of.
+  template <int V>
+  struct Vec {
+    using U = std::conditional_t<V * sizeof(T) == 16, uint4,
+                                 std::conditional_t<V * sizeof(T) == 8, uint2, std::conditional_t<V * sizeof(T) == 4, uint32_t, uint16_t>>>;
+  };
+  template <int V>
+  static __device__ __forceinline__ void store_rows_v(const uint4* s, int lane, T* base, long long ld, int rows, int left) {
+    using U = typename Vec<V>::U;
+    const int c = lane % (32 / V) * V, r0 = lane / (32 / V);
+    T* p = base + r0 * ld + c;
+#pragma unroll 4
+    for (int row = r0; row < 32; row += V, p += V * ld) {
+      const T* e = reinterpret_cast<const T*>(s + slot(row, c / PER)) + c % PER;
+      if (row >= rows) break;
+      if (c + V <= left) {
+        *reinterpret_cast<U*>(p) = *reinterpret_cast<const U*>(e);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (c + i < left) p[i] = e[i];
+      }
+    }
+  }
   static __device__ __forceinline__ void store_rows(const uint4* s, int lane, T* base, long long ld, long long row0, int rows, int col0,
                                                     int cols) {
-    if (col0 + lane >= cols) return;
-    T* p = base + row0 * ld + col0 + lane;
-#pragma unroll 4
-    for (int row = 0; row < rows; ++row) p[row * ld] = reinterpret_cast<const T*>(s + slot(row, lane / PER))[lane % PER];
+    T* p = base + row0 * ld + col0;
+    const uintptr_t step = reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * sizeof(T));
+    if (step % (4 * sizeof(T)) == 0)
+      store_rows_v<4>(s, lane, p, ld, rows, cols - col0);
+    else if (step % (2 * sizeof(T)) == 0)
+      store_rows_v<2>(s, lane, p, ld, rows, cols - col0);
+    else
+      store_rows_v<1>(s, lane, p, ld, rows, cols - col0);
   }
   static __device__ __forceinline__ void load_rows(uint4* s, int lane, const T* base, long long ld, long long row0, int rows, int col0,
                                                    int cols) {
     if (col0 + lane >= cols) return;
     const T* p = base + row0 * ld + col0 + lane;
-#pragma unroll 8
+#pragma unroll 16
     for (int row = 0; row < rows; ++row) reinterpret_cast<T*>(s + slot(row, lane / PER))[lane % PER] = p[row * ld];
   }
 };
@@ -246,7 +294,7 @@ __device__ __forceinline__ void start_residual(const Maps& maps, const WarpStage
 // under way (TMA) and replaced by that of the piece after the next, at next_col
 // (if >= 0). False on a wait that gave up.
 template <class T, bool FULL>
-__device__ __forceinline__ bool finish_piece(const TcArgs& g, const Maps& maps, F2 (&v)[16], WarpStage<T>& w, int lane, long long row0,
+__device__ __forceinline__ bool finish_piece(const Problem& g, const Maps& maps, F2 (&v)[16], WarpStage<T>& w, int lane, long long row0,
                                              int col0, int p, int next_col, volatile int* abort_flag) {
   using P = Piece<T>;
   const Epilogue& e = g.e;
@@ -338,7 +386,7 @@ __device__ __forceinline__ bool finish_piece(const TcArgs& g, const Maps& maps, 
 // The bias of `pieces` times 32 columns into scratch (one float per column), and
 // from there the same values into every lane.
 template <class T, int NP>
-__device__ __forceinline__ void bias_rows(const TcArgs& g, float* scratch, int lane, int col0, F2 (&v)[NP][16]) {
+__device__ __forceinline__ void bias_rows(const Problem& g, float* scratch, int lane, int col0, F2 (&v)[NP][16]) {
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
     const int c = col0 + p * 32 + lane;
@@ -356,9 +404,11 @@ __device__ __forceinline__ void bias_rows(const TcArgs& g, float* scratch, int l
   __syncwarp();
 }
 
-template <class T, bool A_MN, bool B_MN, int BN, bool FULL>
+template <class T, int BN, Kind KIND>
 __global__ void __launch_bounds__(TC_THREADS, 1)
-    gemm_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ TcArgs g) {
+    gemm_tc_kernel(const __grid_constant__ MapSet<kProducts<KIND>> map_set, const __grid_constant__ TcArgs<kProducts<KIND>> args) {
+  constexpr bool FULL = KIND == Kind::forward, TWO = KIND == Kind::gradients, B_MN = !FULL;
+  constexpr int SECOND = TWO ? 1 : 0;
   using C = Cfg<T, BN, FULL>;
   constexpr int NST = C::STAGES;
   extern __shared__ char smem_raw[];
@@ -399,8 +449,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   if (warp == 0 && lane == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b) : "memory");
+    for (int p = 0; p < kProducts<KIND>; ++p) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_set.p[p].a) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_set.p[p].b) : "memory");
+    }
   }
   tc_before();
   __syncthreads();
@@ -411,16 +463,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   prior_done();
 
   constexpr bool PROMOTE = FULL || sizeof(T) == 4;
-  const int tiles = g.tiles_m * g.tiles_n, items = g.whole + (tiles - g.whole) * g.splits;
+  // Items: the whole tiles of both products, then the parts of the others.
+  const int whole0 = args.p[0].whole, whole1 = TWO ? args.p[SECOND].whole : 0;
+  auto parts_of = [&](const Problem& g) { return (g.tiles_m * g.tiles_n - g.whole) * g.splits; };
+  const int parts0 = parts_of(args.p[0]), items = whole0 + whole1 + parts0 + (TWO ? parts_of(args.p[SECOND]) : 0);
   // Tiles in bands of eight tile rows, column after column within a band, so
   // that the clusters running at a time share A's and B's rows in L2.
-  // Returns the index of the part, or -1 for a whole tile.
-  auto place = [&](int item, int& tm, int& tn, int& k0, int& k1) {
-    int t = item, part = -1;
+  // Returns the product; part is the index of the part, or -1 for a whole tile.
+  auto place = [&](int item, int& part, int& tm, int& tn, int& k0, int& k1) {
+    int which = 0, t = item;
+    part = -1;
+    if (TWO && t >= whole0 && t < whole0 + whole1) {
+      which = 1;
+      t -= whole0;
+    } else if (t >= whole0 + whole1) {
+      part = t - whole0 - whole1;
+      if (TWO && part >= parts0) {
+        which = 1;
+        part -= parts0;
+      }
+    }
+    const Problem& g = args.p[TWO ? which : 0];
     k0 = 0;
     k1 = g.kblocks;
-    if (item >= g.whole && g.splits > 1) {
-      part = item - g.whole;
+    if (part >= 0) {
       const int split = part % g.splits;
       t = g.whole + part / g.splits;
       k0 = (int)((long long)g.kblocks * split / g.splits);
@@ -430,9 +496,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int h = min(8, g.tiles_m - band * 8);
     tn = r / h;
     tm = band * 8 + r - tn * h;
-    return part;
+    return which;
   };
-  const int chunk = PROMOTE ? g.chunk : g.kblocks;
+  auto chunk_of = [&](const Problem& g) { return PROMOTE ? g.chunk : g.kblocks; };
 
   if constexpr (PROMOTE) {
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -442,8 +508,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       uint32_t it = 0;
       bool ok = true;
       for (int item = cluster; item < items && ok; item += clusters) {
-        int tm, tn, k0, k1;
-        place(item, tm, tn, k0, k1);
+        int part, tm, tn, k0, k1;
+        const int which = place(item, part, tm, tn, k0, k1);
+        const Problem& g = args.p[TWO ? which : 0];
+        const Maps& maps = map_set.p[TWO ? which : 0];
+        const bool a_mn = KIND == Kind::dweight || (TWO && which == 1);
+        const int chunk = chunk_of(g);
         const int i0 = tm * 256 + (int)rank * 128, j0 = tn * BN + (int)rank * (BN / 2);
         // a chunk of k blocks of every plane pair, chunk after chunk
         int c0 = k0, seg = 0, kb = k0;
@@ -457,7 +527,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           const uint32_t lbar = leader_addr(full(s));
           if (rank == 0) expect_tx(full(s), 2 * C::STAGE);
           const int x = kb * KB, pa = g.pa[seg], pb = g.pb[seg];
-          if (A_MN) {
+          if (a_mn) {
             tma_load(a, &maps.a, i0, x, pa, lbar);
             tma_load(a + 8192, &maps.a, i0 + 64, x, pa, lbar);
           } else {
@@ -483,15 +553,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
       // float32 accumulator, both operands of one 16-bit type, M = 256 over the pair
-      const uint32_t ab = g.f16 ? 0u : 1u;
-      const uint32_t idesc = (1u << 4) | (ab << 7) | (ab << 10) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
-                             ((uint32_t)(BN >> 3) << 17) | (16u << 24);
-      const uint64_t ad0 = desc_base(A_MN ? 8192 : 16), bd0 = desc_base(B_MN ? 8192 : 16);
+      const uint32_t ab = args.f16 ? 0u : 1u;
+      const uint32_t idesc0 = (1u << 4) | (ab << 7) | (ab << 10) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | (16u << 24);
+      const uint64_t bd0 = desc_base(B_MN ? 8192 : 16);
       uint32_t it = 0, n_acc = 0;
       bool ok = true;
       for (int item = cluster; item < items && ok; item += clusters) {
-        int tm, tn, k0, k1;
-        place(item, tm, tn, k0, k1);
+        int part, tm, tn, k0, k1;
+        const int which = place(item, part, tm, tn, k0, k1);
+        const Problem& g = args.p[TWO ? which : 0];
+        const bool a_mn = KIND == Kind::dweight || (TWO && which == 1);
+        const int chunk = chunk_of(g);
+        const uint32_t idesc = idesc0 | ((a_mn ? 1u : 0u) << 15), a_step = a_mn ? 128 : 2;
+        const uint64_t ad0 = desc_base(a_mn ? 8192 : 16);
         for (int c0 = k0; c0 < k1 && ok; c0 += chunk, ++n_acc) {
           const int buf = n_acc & 1, steps = (min(c0 + chunk, k1) - c0) * g.segments;
           if (!mbar_wait(acce(buf), ((n_acc >> 1) & 1) ^ 1, abort_flag, 21)) {
@@ -511,7 +585,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             const uint64_t ad = ad0 | ((a >> 4) & 0x3FFF), bd = bd0 | ((b >> 4) & 0x3FFF);
 #pragma unroll
             for (int q = 0; q < KB / 16; ++q)  // 16 k values: 32 bytes along a row, or two 8-k groups
-              mma_f16_pair(acc, ad + q * (A_MN ? 128 : 2), bd + q * (B_MN ? 128 : 2), idesc, (k > 0 || q > 0) ? 1u : 0u);
+              mma_f16_pair(acc, ad + q * a_step, bd + q * (B_MN ? 128 : 2), idesc, (k > 0 || q > 0) ? 1u : 0u);
             commit_pair(empty(s));
           }
           commit_pair(accf(buf));
@@ -533,8 +607,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     uint32_t n_acc = 0;
     bool ok = true;
     for (int item = cluster; item < items && ok; item += clusters) {
-      int tm, tn, k0, k1;
-      const int part = place(item, tm, tn, k0, k1);
+      int part, tm, tn, k0, k1;
+      const int which = place(item, part, tm, tn, k0, k1);
+      const Problem& g = args.p[TWO ? which : 0];
+      const Maps& maps = map_set.p[TWO ? which : 0];
+      const int chunk = chunk_of(g);
       const long long row0 = (long long)tm * 256 + rank * 128 + quad * 32;
       const int cols0 = tn * BN + half * (BN / 2);
       const bool live = row0 < g.m && cols0 < g.n;
@@ -652,10 +729,13 @@ __device__ __forceinline__ void store_some(T* p, const float (&v)[4], int count,
       if (i < count) p[i] = Elem<T>::from_f(v[i]);
   }
 }
-template <class T, bool FULL>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs g, int bn) {
+template <class T, bool FULL, int N>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArgs<N> args, int bn) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = g.whole + blockIdx.y, band = t / (8 * g.tiles_n), r0 = t - band * 8 * g.tiles_n;
+  const int rest0 = args.p[0].tiles_m * args.p[0].tiles_n - args.p[0].whole;
+  const int which = N == 2 && (int)blockIdx.y >= rest0 ? 1 : 0, nth = (int)blockIdx.y - (which ? rest0 : 0);
+  const Problem& g = args.p[N == 2 ? which : 0];
+  const int t = g.whole + nth, band = t / (8 * g.tiles_n), r0 = t - band * 8 * g.tiles_n;
   const int h = min(8, g.tiles_m - band * 8), tn = r0 / h, tm = band * 8 + r0 - tn * h;
   const int piece = blockIdx.x, strip = piece / (bn / 32), cp = piece - strip * (bn / 32);
   const int r = warp * 4 + (lane & 3), quad = lane >> 2;
@@ -667,7 +747,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcArg
   const bool live = row < g.m;
   const Epilogue& e = g.e;
   const size_t part_size = (size_t)64 * bn;  // float4s of a partial tile
-  const float4* p = reinterpret_cast<const float4*>(g.partial) + (size_t)blockIdx.y * g.splits * part_size + (size_t)piece * 256 + quad * 32 + r;
+  const float4* p = reinterpret_cast<const float4*>(g.partial) + (size_t)nth * g.splits * part_size + (size_t)piece * 256 + quad * 32 + r;
   float v[4] = {0.f, 0.f, 0.f, 0.f}, bias[4] = {0.f, 0.f, 0.f, 0.f}, res[4] = {0.f, 0.f, 0.f, 0.f};
   if (FULL && live) {
     if (e.bias) {
@@ -771,102 +851,199 @@ static bool make_piece_map(CUtensorMap* map, const void* p, long long rows, int 
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tile width, the tiles that run whole, and the k splits of the others.
+// Sizes of a product: (m, k) x (n, k) in `segments` plane pairs.
+struct Size {
+  long long m;
+  int n, kblocks, segments;
+};
+// Tile width and, for each product, the tiles that run whole and the k splits of
+// the others.
 struct Schedule {
-  int bn, tiles_m, tiles_n, whole, splits;
+  int bn, tiles_m[2], tiles_n[2], whole[2], splits[2];
+  double clocks;
+  int rest(int p) const { return tiles_m[p] * tiles_n[p] - whole[p]; }
 };
 constexpr int PAIRS = 74;  // SM pairs
+constexpr int kMostSplits = 64;
 // Least estimated time, in SM clocks. A k block takes 560 clocks for 256 columns
 // and 440 for 128 (32 and 24 KB per SM, at the 55 to 58 bytes per clock that L2
 // delivers to an SM: measured 566 and 444 on 4096 x 4096 x 11008), a tile 2500
-// more that nothing hides. Tiles beyond whole waves may be split: then their parts
-// fill waves of their own, and the partial tiles' way through L2 and a second
-// launch come on top.
-static Schedule schedule_for(long long m, int n, int kblocks, int segments) {
+// more that nothing hides. One product: tiles beyond whole waves may be split;
+// then their parts fill waves of their own, and the partial tiles' way through L2
+// and a second launch come on top. Two products: all tiles of one or both may be
+// split, into parts of about the same length.
+static Schedule schedule_for(const Size* p, int count) {
   Schedule best{};
-  double least = 1e300;
+  best.clocks = 1e300;
   for (int bn : {256, 128}) {
-    const long long tm = (m + 255) / 256, tn = (n + bn - 1) / bn, tiles = tm * tn;
-    const double block = (bn == 256 ? 560.0 : 440.0) * segments, tile = kblocks * block + 2500.0;
-    const long long whole = tiles / PAIRS * PAIRS, rest = tiles - whole;
-    for (int s = 1; s <= 16 && (s == 1 || (kblocks / s >= 2 && rest)); ++s) {
-      double t = whole / PAIRS * tile;
-      if (s == 1)
-        t += rest ? tile : 0.0;
-      else
-        t += (rest * s + PAIRS - 1) / PAIRS * (((kblocks + s - 1) / s) * block + 2500.0) + 5000.0 + (double)rest * (s + 1) * 256 * bn * 4 / 2500.0;
-      if (t < least) {
-        least = t;
-        best = {bn, (int)tm, (int)tn, (int)(s == 1 ? tiles : whole), s};
+    Schedule s{};
+    s.bn = bn;
+    double block[2] = {0, 0};
+    long long tiles[2] = {0, 0};
+    for (int i = 0; i < count; ++i) {
+      s.tiles_m[i] = (int)((p[i].m + 255) / 256);
+      s.tiles_n[i] = (p[i].n + bn - 1) / bn;
+      tiles[i] = (long long)s.tiles_m[i] * s.tiles_n[i];
+      block[i] = (bn == 256 ? 560.0 : 440.0) * p[i].segments;
+    }
+    auto part = [&](int i, int splits) { return ((p[i].kblocks + splits - 1) / splits) * block[i] + 2500.0; };
+    auto joins = [&](int i, long long rest, int splits) { return splits > 1 ? (double)rest * (splits + 1) * 256 * bn * 4 / 2500.0 + 120.0 * splits : 0.0; };
+    auto consider = [&](double t) {
+      if (t < best.clocks) {
+        best = s;
+        best.clocks = t;
+      }
+    };
+    if (count == 1) {
+      const long long whole = tiles[0] / PAIRS * PAIRS, rest = tiles[0] - whole;
+      for (int n = 1; n <= kMostSplits && (n == 1 || (p[0].kblocks / n >= 2 && rest && rest * n <= 8 * PAIRS)); ++n) {
+        s.whole[0] = (int)(n == 1 ? tiles[0] : whole);
+        s.splits[0] = n;
+        consider(whole / PAIRS * part(0, 1) + (rest * n + PAIRS - 1) / PAIRS * part(0, n) + (n > 1 ? 5000.0 + joins(0, rest, n) : 0.0));
+      }
+      continue;
+    }
+    for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      // the first product in n parts, the second in parts of about their length
+      const double steps = (double)((p[0].kblocks + n - 1) / n) * p[0].segments;
+      int n1 = (int)((double)p[1].kblocks * p[1].segments / steps + 0.5);
+      n1 = n1 < 1 ? 1 : n1 > kMostSplits ? kMostSplits : n1;
+      if (n1 > 1 && p[1].kblocks / n1 < 2) n1 = p[1].kblocks / 2 > 0 ? p[1].kblocks / 2 : 1;
+      if (n > 1 && p[0].kblocks / n < 2) break;
+      s.splits[0] = n;
+      s.splits[1] = n1;
+      s.whole[0] = n == 1 ? (int)tiles[0] : 0;
+      s.whole[1] = n1 == 1 ? (int)tiles[1] : 0;
+      const double longest = part(0, n) > part(1, n1) ? part(0, n) : part(1, n1);
+      const long long items = tiles[0] * n + tiles[1] * n1;
+      double t = items <= PAIRS ? longest : (tiles[0] * n * part(0, n) + tiles[1] * n1 * part(1, n1)) / PAIRS + 0.5 * longest;
+      if (n > 1 || n1 > 1) t += 5000.0 + joins(0, tiles[0], n) + joins(1, tiles[1], n1);
+      if ((n == 1 && n1 == 1) || items <= 8 * PAIRS) consider(t);  // a bound for the workspace
+      if (n1 > 1 && n == 1) {  // neither
+        s.splits[1] = 1;
+        s.whole[1] = (int)tiles[1];
+        const double far = part(0, 1) > part(1, 1) ? part(0, 1) : part(1, 1);
+        consider(tiles[0] + tiles[1] <= PAIRS ? far : (tiles[0] * part(0, 1) + tiles[1] * part(1, 1)) / PAIRS + 0.5 * far);
       }
     }
   }
   return best;
 }
-static size_t partial_bytes(long long m, int n, int kblocks, int segments) {
-  const Schedule s = schedule_for(m, n, kblocks, segments);
-  return (size_t)(s.tiles_m * s.tiles_n - s.whole) * s.splits * 256 * s.bn * sizeof(float);
+static size_t partial_bytes(const Schedule& s, int p) { return (size_t)s.rest(p) * s.splits[p] * 256 * s.bn * sizeof(float); }
+// Whether two products go into one launch: their tiles then share the waves and
+// one launch of partial tiles' sums, which small products gain from (394 x 520 ->
+// 1000 in float32 38.7 -> 30.1 us); of long ones some clusters get a long tile
+// more than others, and 4096 x 4096 -> 11008 in bfloat16 takes 660 us in one
+// launch, 628 in two.
+static bool together(const Size* p) {
+  return schedule_for(p, 2).clocks < schedule_for(p, 1).clocks + schedule_for(p + 1, 1).clocks + 5000.0;
+}
+static size_t partial_bytes(const Size* p, int count) {
+  if (count == 2 && !together(p)) {
+    const size_t a = partial_bytes(p, 1), b = partial_bytes(p + 1, 1);
+    return a > b ? a : b;
+  }
+  const Schedule s = schedule_for(p, count);
+  size_t n = 0;
+  for (int i = 0; i < count; ++i) n += partial_bytes(s, i);
+  return n;
 }
 static int plane_pairs(int planes_a, int planes_b) { return planes_a == 1 ? planes_b : planes_b == 1 ? planes_a : 6; }
 
-template <class T, bool A_MN, bool B_MN, int BN, bool FULL>
-static cudaError_t launch_tc_t(const Maps& maps, const TcArgs& g, cudaStream_t st) {
-  auto kern = gemm_tc_kernel<T, A_MN, B_MN, BN, FULL>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (Cfg<T, BN, FULL>::SMEM));
+// A product to launch: C (m, n) with its epilogue.
+struct Product {
+  Operand a, b;
+  long long m, k;
+  int n;
+  Epilogue e;
+  Size size() const { return {m, n, (int)((k + KB - 1) / KB), plane_pairs(a.planes, b.planes)}; }
+};
+
+template <class T, int BN, Kind KIND>
+static cudaError_t launch_tc_t(const MapSet<kProducts<KIND>>& maps, const TcArgs<kProducts<KIND>>& g, int items, int rest, cudaStream_t st) {
+  constexpr bool FULL = KIND == Kind::forward;
+  constexpr int smem = Cfg<T, BN, FULL>::SMEM;
+  auto kern = gemm_tc_kernel<T, BN, KIND>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int rest = g.tiles_m * g.tiles_n - g.whole;
-  const long long items = g.whole + (long long)rest * g.splits;
-  e = launch_overlapped(kern, (unsigned)(2 * (items < PAIRS ? items : PAIRS)), TC_THREADS, (Cfg<T, BN, FULL>::SMEM), st, 2, maps, g);
+  e = launch_overlapped(kern, (unsigned)(2 * (items < PAIRS ? items : PAIRS)), TC_THREADS, smem, st, 2, maps, g);
   if (e == cudaSuccess && rest > 0)
-    e = launch_overlapped(join_kernel<T, FULL>, dim3(BN / 32 * 8, rest), 256, 0, st, 1, g, BN);
+    e = launch_overlapped(join_kernel<T, FULL, kProducts<KIND>>, dim3(BN / 32 * 8, rest), 256, 0, st, 1, g, BN);
   return e;
 }
 
-// dtype: of the result and the epilogue's tensors; operands of a float32
-// product are bfloat16 planes. partial: partial_bytes() of workspace.
-static cudaError_t launch_tc(const Operand& a, const Operand& b, long long m, int n, long long k, const Epilogue& e, int dtype,
-                             float* partial, cudaStream_t st) {
+// The products of one launch. dtype: of the results and the epilogue's tensors;
+// operands of a float32 product are bfloat16 planes. partial: partial_bytes() of
+// workspace.
+template <Kind KIND>
+static cudaError_t launch_tc(const Product* products, int dtype, float* partial, cudaStream_t st) {
   if (!encode_tiled()) return cudaErrorNotSupported;
-  TcArgs g{};
-  g.m = (int)m;
-  g.n = n;
-  g.kblocks = (int)((k + KB - 1) / KB);
-  g.segments = plane_pairs(a.planes, b.planes);
-  static const uint8_t six_a[6] = {2, 0, 1, 1, 0, 0}, six_b[6] = {0, 2, 1, 0, 1, 0};
-  for (int s = 0; s < g.segments; ++s) {
-    g.pa[s] = b.planes == 1 ? g.segments - 1 - s : a.planes == 1 ? 0 : six_a[s];
-    g.pb[s] = a.planes == 1 ? g.segments - 1 - s : b.planes == 1 ? 0 : six_b[s];
-  }
-  g.chunk = dtype == SCMP_F32 ? 4 : 16;
-  const Schedule sc = schedule_for(m, n, g.kblocks, g.segments);
-  g.tiles_m = sc.tiles_m;
-  g.tiles_n = sc.tiles_n;
-  g.whole = sc.whole;
-  g.splits = sc.splits;
-  g.f16 = dtype == SCMP_F16;
-  g.partial = partial;
-  g.e = e;
+  constexpr int N = kProducts<KIND>;
+  Size sizes[N];
+  for (int i = 0; i < N; ++i) sizes[i] = products[i].size();
+  const Schedule sc = schedule_for(sizes, N);
+  TcArgs<N> args{};
+  MapSet<N> maps;
+  args.f16 = dtype == SCMP_F16;
   const size_t es = dtype_size(dtype);
-  g.tma_out = rows_aligned16(e.out, e.ldo, es);
-  g.tma_res = e.residual && rows_aligned16(e.residual, e.ldr, es);
-  g.tma_pre = e.pre && rows_aligned16(e.pre, n, es);
-  g.vec_codes = aligned16(e.codes) && n % 16 == 0;
-  g.vec_out = rows_aligned4(e.out, e.ldo, es);
-  g.vec_pre = rows_aligned4(e.pre, n, es);
-  Maps maps;
-  if (!make_map(&maps.a, a, g.f16, 128) || !make_map(&maps.b, b, g.f16, sc.bn / 2) ||
-      (g.tma_out && !make_piece_map(&maps.out, e.out, m, n, e.ldo, dtype)) ||
-      (g.tma_res && !make_piece_map(&maps.res, e.residual, m, n, e.ldr, dtype)) ||
-      (g.tma_pre && !make_piece_map(&maps.pre, e.pre, m, n, n, dtype)))
-    return cudaErrorInvalidValue;
+  int items = 0, rest = 0;
+  for (int i = 0; i < N; ++i) {
+    const Product& p = products[i];
+    const Epilogue& e = p.e;
+    Problem& g = args.p[i];
+    Maps& m = maps.p[i];
+    g.m = (int)p.m;
+    g.n = p.n;
+    g.kblocks = sizes[i].kblocks;
+    g.segments = sizes[i].segments;
+    static const uint8_t six_a[6] = {2, 0, 1, 1, 0, 0}, six_b[6] = {0, 2, 1, 0, 1, 0};
+    for (int s = 0; s < g.segments; ++s) {
+      g.pa[s] = p.b.planes == 1 ? g.segments - 1 - s : p.a.planes == 1 ? 0 : six_a[s];
+      g.pb[s] = p.a.planes == 1 ? g.segments - 1 - s : p.b.planes == 1 ? 0 : six_b[s];
+    }
+    g.chunk = dtype == SCMP_F32 ? 4 : 16;
+    g.tiles_m = sc.tiles_m[i];
+    g.tiles_n = sc.tiles_n[i];
+    g.whole = sc.whole[i];
+    g.splits = sc.splits[i];
+    g.partial = partial;
+    partial += partial_bytes(sc, i) / sizeof(float);
+    g.e = e;
+    g.tma_out = rows_aligned16(e.out, e.ldo, es);
+    g.tma_res = e.residual && rows_aligned16(e.residual, e.ldr, es);
+    g.tma_pre = e.pre && rows_aligned16(e.pre, p.n, es);
+    g.vec_codes = aligned16(e.codes) && p.n % 16 == 0;
+    g.vec_out = rows_aligned4(e.out, e.ldo, es);
+    g.vec_pre = rows_aligned4(e.pre, p.n, es);
+    if (!make_map(&m.a, p.a, args.f16, 128) || !make_map(&m.b, p.b, args.f16, sc.bn / 2) ||
+        (g.tma_out && !make_piece_map(&m.out, e.out, p.m, p.n, e.ldo, dtype)) ||
+        (g.tma_res && !make_piece_map(&m.res, e.residual, p.m, p.n, e.ldr, dtype)) ||
+        (g.tma_pre && !make_piece_map(&m.pre, e.pre, p.m, p.n, p.n, dtype)))
+      return cudaErrorInvalidValue;
+    items += g.whole + sc.rest(i) * g.splits;
+    rest += sc.rest(i);
+  }
   return with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    if (!a.mn && !b.mn)
-      return sc.bn == 256 ? launch_tc_t<T, false, false, 256, true>(maps, g, st) : launch_tc_t<T, false, false, 128, true>(maps, g, st);
-    if (!a.mn)
-      return sc.bn == 256 ? launch_tc_t<T, false, true, 256, false>(maps, g, st) : launch_tc_t<T, false, true, 128, false>(maps, g, st);
-    return sc.bn == 256 ? launch_tc_t<T, true, true, 256, false>(maps, g, st) : launch_tc_t<T, true, true, 128, false>(maps, g, st);
+    return sc.bn == 256 ? launch_tc_t<T, 256, KIND>(maps, args, items, rest, st) : launch_tc_t<T, 128, KIND>(maps, args, items, rest, st);
   });
+}
+// The gradients dx (null: none) and dweight (null: none), in one launch or, one
+// after the other, in two; the second then overwrites the first's partial tiles
+// when that has finished.
+static cudaError_t launch_gradients(const Product* dx, const Product* dw, int dtype, float* partial, cudaStream_t st) {
+  if (dx && dw) {
+    const Size sizes[2] = {dx->size(), dw->size()};
+    if (together(sizes)) {
+      const Product both[2] = {*dx, *dw};
+      return launch_tc<Kind::gradients>(both, dtype, partial, st);
+    }
+  }
+  if (dx) {
+    const cudaError_t e = launch_tc<Kind::dx>(dx, dtype, partial, st);
+    if (e != cudaSuccess) return e;
+  }
+  return dw ? launch_tc<Kind::dweight>(dw, dtype, partial, st) : cudaSuccess;
 }
 
 // ---------------------------------------------------------------------------
