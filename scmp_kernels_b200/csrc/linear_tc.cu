@@ -65,9 +65,10 @@ struct Cfg {
   static constexpr int PIECE = 32 * 32 * sizeof(T);          // a 32 x 32 piece of the result
   static constexpr int RES = FULL ? 2 : 0;                   // pieces of the residual on their way
   static constexpr int STG = EPI_WARPS * (2 + RES) * PIECE;  // per epilogue warp: two pieces of the result as well
-  static constexpr int STAGES = (227 * 1024 - 1536 - STG) / STAGE;
+  static constexpr int STAGES = (227 * 1024 - 1536 - 1024 - STG) / STAGE;
   static constexpr int NP = BN / 64;            // 32-column pieces per epilogue warp
-  static constexpr int SMEM = STAGES * STAGE + STG + 512 + 1024;
+  static constexpr int BIAS = FULL && sizeof(T) == 2 ? 2 * 256 * 2 : 0;  // two tiles' bias
+  static constexpr int SMEM = STAGES * STAGE + STG + BIAS + 512 + 1024;
 };
 
 // What a launch computes. The forward pass's product has k-contiguous operands and
@@ -383,6 +384,21 @@ __device__ __forceinline__ bool finish_piece(const Problem& g, const Maps& maps,
   }
   return true;
 }
+// 32 columns' bias, in shared memory in T, added to every lane's row.
+template <class T>
+__device__ __forceinline__ void add_bias(const uint16_t* s, F2 (&v)[16]) {
+  if constexpr (sizeof(T) == 2) {
+    const T* t = nullptr;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint4 b = reinterpret_cast<const uint4*>(s)[q];
+      v[4 * q] = add2(unpack_pair(b.x, t), v[4 * q]);
+      v[4 * q + 1] = add2(unpack_pair(b.y, t), v[4 * q + 1]);
+      v[4 * q + 2] = add2(unpack_pair(b.z, t), v[4 * q + 2]);
+      v[4 * q + 3] = add2(unpack_pair(b.w, t), v[4 * q + 3]);
+    }
+  }
+}
 // The bias of `pieces` times 32 columns into scratch (one float per column), and
 // from there the same values into every lane.
 template <class T, int NP>
@@ -414,7 +430,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   extern __shared__ char smem_raw[];
   char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(base);
-  char* tail = base + NST * C::STAGE + C::STG;
+  char* tail = base + NST * C::STAGE + C::STG + C::BIAS;
   const uint32_t bars = smem_u32(tail);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail + 8 * (2 * NST + 5 + 2 * EPI_WARPS));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 8 * (2 * NST + 5 + 2 * EPI_WARPS) + 4);
@@ -633,52 +649,96 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
       };
       if constexpr (PROMOTE) {
+        // A tile of one chain is read piece by piece: no sums to hold and choose from
+        // (12608 x 768 -> 768 float16 with bias and residual 27.4 -> 25.7 us, without
+        // 20.5 -> 18.8 us; with the bias read from memory 27.6). A bias of the result's type
+        // waits in shared memory meanwhile, where this half's four warps put the same
+        // values; the slot is free again two tiles on, since the MMAs of that tile began
+        // when every warp had read its accumulator.
+        const bool biased = FULL && g.e.bias && part < 0;
+        const bool one = k1 - k0 <= chunk && (!biased || (sizeof(T) == 2 && !g.e.bias_f32));
+        uint16_t* bias = reinterpret_cast<uint16_t*>(base + NST * C::STAGE + C::STG) + (n_acc & 1) * 256 + half * 128;
+        const uint32_t src0 = tmem + lanes + half * (BN / 2);
         F2 sum[C::NP][16];
-        if (FULL && g.e.bias && part < 0) {
-          if (lane == 0) tma_store_read();
-          __syncwarp();
-          bias_rows<T>(g, reinterpret_cast<float*>(ws.out(0)), lane, cols0, sum);
-        } else {
+        if (one) {
+          uint16_t b[C::NP] = {};
+          if (biased) {
 #pragma unroll
-          for (int p = 0; p < C::NP; ++p)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sum[p][j] = f2(0.f);
-        }
-        for (int c0 = k0; c0 < k1; c0 += chunk, ++n_acc) {
-          const int buf = n_acc & 1;
-          if (!mbar_wait(accf(buf), (n_acc >> 1) & 1, abort_flag, 24)) {
-            ok = false;
-            break;
+            for (int p = 0; p < C::NP; ++p) {
+              const int c = cols0 + p * 32 + lane;
+              if (c < g.n) b[p] = __ldg((const unsigned short*)g.e.bias + c);
+            }
           }
+          if (!mbar_wait(accf(n_acc & 1), (n_acc >> 1) & 1, abort_flag, 24)) break;
           tc_after();
-          const uint32_t src = tmem + lanes + buf * ACC_COLS + half * (BN / 2);
-          // the next 16 columns are on their way while these are added
-          uint32_t r[2][16];
-          tmem_ld16(src, r[0]);
+          if (biased) {
 #pragma unroll
-          for (int q = 0; q < 2 * C::NP; ++q) {
-            tmem_wait();
-            if (q + 1 < 2 * C::NP) tmem_ld16(src + (q + 1) * 16, r[(q + 1) & 1]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              sum[q >> 1][(q & 1) * 8 + j] = add2(sum[q >> 1][(q & 1) * 8 + j], f2(__uint_as_float(r[q & 1][2 * j]), __uint_as_float(r[q & 1][2 * j + 1])));
+            for (int p = 0; p < C::NP; ++p) bias[p * 32 + lane] = b[p];
+            __syncwarp();
           }
-          tc_before();  // the accumulator is read: the MMAs may overwrite it
-          __syncwarp();
-          if (lane == 0) arrive_cluster(leader_addr(acce(buf)));
+        } else {
+          if (biased) {
+            if (lane == 0) tma_store_read();
+            __syncwarp();
+            bias_rows<T>(g, reinterpret_cast<float*>(ws.out(0)), lane, cols0, sum);
+          } else {
+#pragma unroll
+            for (int p = 0; p < C::NP; ++p)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) sum[p][j] = f2(0.f);
+          }
+          for (int c0 = k0; c0 < k1; c0 += chunk, ++n_acc) {
+            const int buf = n_acc & 1;
+            if (!mbar_wait(accf(buf), (n_acc >> 1) & 1, abort_flag, 24)) {
+              ok = false;
+              break;
+            }
+            tc_after();
+            const uint32_t src = src0 + buf * ACC_COLS;
+            // the next 16 columns are on their way while these are added
+            uint32_t h[2][16];
+            tmem_ld16(src, h[0]);
+#pragma unroll
+            for (int q = 0; q < 2 * C::NP; ++q) {
+              tmem_wait();
+              if (q + 1 < 2 * C::NP) tmem_ld16(src + (q + 1) * 16, h[(q + 1) & 1]);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                sum[q >> 1][(q & 1) * 8 + j] = add2(sum[q >> 1][(q & 1) * 8 + j], f2(__uint_as_float(h[q & 1][2 * j]), __uint_as_float(h[q & 1][2 * j + 1])));
+            }
+            tc_before();  // the accumulator is read: the MMAs may overwrite it
+            __syncwarp();
+            if (lane == 0) arrive_cluster(leader_addr(acce(buf)));
+          }
         }
         // one copy of the epilogue's code, which would not fit the instruction cache four times
 #pragma unroll 1
         for (int p = 0; p < C::NP && ok; ++p) {
           F2 v[16];
+          if (one) {
+            const int buf = n_acc & 1;
+            uint32_t r[32];
+            tmem_ld32(src0 + buf * ACC_COLS + p * 32, r);
+            tmem_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            v[j] = sum[0][j];
+            for (int j = 0; j < 16; ++j) v[j] = f2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+            if (biased) add_bias<T>(bias + p * 32, v);
+            if (p == C::NP - 1) {
+              tc_before();
+              __syncwarp();
+              if (lane == 0) arrive_cluster(leader_addr(acce(buf)));
+            }
+          } else {
 #pragma unroll
-            for (int i = 1; i < C::NP; ++i) v[j] = p == i ? sum[i][j] : v[j];
+            for (int j = 0; j < 16; ++j) {
+              v[j] = sum[0][j];
+#pragma unroll
+              for (int i = 1; i < C::NP; ++i) v[j] = p == i ? sum[i][j] : v[j];
+            }
           }
           emit(p, v);
         }
+        if (one) ++n_acc;
       } else {
         const int buf = n_acc & 1;
         if (!mbar_wait(accf(buf), (n_acc >> 1) & 1, abort_flag, 24)) break;
