@@ -663,3 +663,44 @@ def test_small_workspaces_are_refused():
     st = lib.scmp_linear_backward(x.data_ptr(), 64, x.data_ptr(), 64, None, None, x.data_ptr(), 64, x.data_ptr(), 64,
                                   None, None, _lib.F32, 4, 64, 64, 1, x.data_ptr(), None, None, _lib.F32, None, 0, None)
     assert st == _lib.SCMP_ERR_WORKSPACE and b"workspace" in lib.scmp_last_error()
+
+
+# ---------------------------------------------------------------------------
+# linear: many tiles, split tiles, odd pitches
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(5000, 130, 2600), (4500, 64, 2601), (2600, 1100, 1999), (300, 2500, 40)])
+def test_linear_forward_of_many_tiles(dtype, shape):
+    # several tiles of different columns in turn on every SM pair, with one accumulator
+    # chain and with more; the last of few tiles in parts
+    t, (r, d, m) = DT[dtype], shape
+    x, w, b, res = lin_inputs(shape, t, 60)
+    pre64 = x.double() @ w.double().t()
+    _, pb = product_bounds(x.double(), w.double().t(), d)
+    for bias in (b.to(t), b, None):
+        p64 = pre64 if bias is None else pre64 + bias.double()
+        for residual in (res, None):
+            want = p64 if residual is None else p64 + residual.double()
+            y = S.linear_forward(x, w, bias, residual=residual)
+            close(y, want, U[t] * want.abs() + TINY[t] + pb + 2 * E * p64.abs() + 2 * E * want.abs())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(700, 1024, 1030), (394, 520, 1000), (300, 600, 5000), (12340, 320, 256),
+                                   (40, 4000, 4100), (3000, 44, 300), (3000, 46, 300), (3000, 45, 301)])
+def test_linear_gradients_together_and_alone(dtype, shape):
+    t, (r, d, m) = DT[dtype], shape
+    x, w, _, _ = lin_inputs(shape, t, 61)
+    dy = randn(gen(62), r, m, dtype=t)
+    dy64 = dy.double()
+    dx64, dw64 = dy64 @ w.double(), dy64.t() @ x.double()
+    _, xb = product_bounds(dy64, w.double(), m)
+    _, wb = product_bounds(dy64.t(), x.double(), r)
+    both = S.linear_backward(dy, x, w, with_bias=False)
+    alone = (S.linear_backward(dy, None, w, need_dweight=False, with_bias=False)[0],
+             S.linear_backward(dy, x, None, need_dx=False, with_bias=False)[1])
+    for dx, dw in (both[:2], alone):
+        close(dx, dx64, U[t] * dx64.abs() + TINY[t] + xb)
+        close(dw, dw64, U[t] * dw64.abs() + TINY[t] + wb)
+    again = S.linear_backward(dy, x, w, with_bias=False)
+    assert torch.equal(again[0], both[0]) and torch.equal(again[1], both[1])
