@@ -262,7 +262,7 @@ static ForwardPlan plan_forward(Carve& c, int dtype, long long rows, int d, int 
   const bool f32 = dtype == SCMP_F32;
   if (f32 || (unal & kUnalignedX)) p.x = c.take<char>(staged_bytes(planes_of(dtype), rows, d));
   if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(planes_of(dtype), m, d));
-  const Size size{rows, m, cdiv(d, KB), f32 ? 6 : 1};
+  const Size size{rows, m, cdiv(d, KB), f32 ? 6 : 1, false};
   p.partial = c.take<char>(partial_bytes(&size, 1));
   return p;
 }
@@ -285,14 +285,14 @@ static BackwardPlan plan_backward(Carve& c, int dtype, long long rows, int d, in
   int count = 0;
   if (parts & 1) {
     if (f32 || (unal & kUnalignedWeight)) p.w = c.take<char>(staged_bytes(planes_of(dtype), m, d));
-    sizes[count++] = {rows, d, cdiv(m, KB), plane_pairs(p.planes, f32 ? 3 : 1)};
+    sizes[count++] = {rows, d, cdiv(m, KB), plane_pairs(p.planes, f32 ? 3 : 1), true};
   }
   if (parts & 2) {
     if (x8)
       p.x = c.take<char>(staged_bytes(1, rows, d));
     else if (f32 || (unal & kUnalignedX))
       p.x = c.take<char>(staged_bytes(planes_of(dtype), rows, d));
-    sizes[count++] = {m, d, (int)((rows + KB - 1) / KB), plane_pairs(p.planes, f32 && !x8 ? 3 : 1)};
+    sizes[count++] = {m, d, (int)((rows + KB - 1) / KB), plane_pairs(p.planes, f32 && !x8 ? 3 : 1), true};
   }
   if (count) p.partial = c.take<char>(partial_bytes(sizes, count));
   if (parts & 4) p.part = c.take<float>((size_t)p.row_blocks * m);

@@ -281,6 +281,7 @@ struct WarpStage {
   uint4* base;      // out 0, out 1, residual 0, residual 1
   uint32_t bars;    // of residual 0 and 1
   uint32_t phases;  // bit b: the phase residual b waits for
+  int turn;         // the result's next piece
   __device__ __forceinline__ uint4* out(int b) const { return base + b * (Piece<T>::PIECES * 32); }
   __device__ __forceinline__ uint4* res(int b) const { return base + (2 + b) * (Piece<T>::PIECES * 32); }
 };
@@ -300,7 +301,8 @@ __device__ __forceinline__ bool finish_piece(const Problem& g, const Maps& maps,
   using P = Piece<T>;
   const Epilogue& e = g.e;
   const int rows = (int)(g.m - row0 < 32 ? g.m - row0 : 32);
-  uint4* out = w.out(p & 1);
+  uint4* out = w.out(w.turn);
+  w.turn ^= 1;
   if (lane == 0) {  // the piece that was in the buffer has left
     if (FULL && e.pre)
       tma_store_read();
@@ -618,7 +620,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if constexpr (PROMOTE) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int ew = warp - 4, quad = ew & 3, half = ew >> 2;
     char* stg = base + NST * C::STAGE + ew * (2 + C::RES) * C::PIECE;
-    WarpStage<T> ws{reinterpret_cast<uint4*>(stg), drain + 8 + 16 * ew, 0};
+    WarpStage<T> ws{reinterpret_cast<uint4*>(stg), drain + 8 + 16 * ew, 0, 0};
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     uint32_t n_acc = 0;
     bool ok = true;
@@ -651,7 +653,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       if constexpr (PROMOTE) {
         // A tile of one chain is read piece by piece: no sums to hold and choose from
         // (12608 x 768 -> 768 float16 with bias and residual 27.4 -> 25.7 us, without
-        // 20.5 -> 18.8 us; with the bias read from memory 27.6). A bias of the result's type
+        // 20.5 -> 18.8 us, 256-wide tiles; with the bias read from memory 27.6). A bias of the result's type
         // waits in shared memory meanwhile, where this half's four warps put the same
         // values; the slot is free again two tiles on, since the MMAs of that tile began
         // when every warp had read its accumulator.
@@ -915,6 +917,7 @@ static bool make_piece_map(CUtensorMap* map, const void* p, long long rows, int 
 struct Size {
   long long m;
   int n, kblocks, segments;
+  bool b_mn;  // B's tile axis is contiguous
 };
 // Tile width and, for each product, the tiles that run whole and the k splits of
 // the others.
@@ -925,17 +928,20 @@ struct Schedule {
 };
 constexpr int PAIRS = 74;  // SM pairs
 constexpr int kMostSplits = 64;
-// Least estimated time, in SM clocks. A k block takes 560 clocks for 256 columns
-// and 440 for 128 (32 and 24 KB per SM, at the 55 to 58 bytes per clock that L2
+// Least estimated time, in SM clocks. A k block takes 560 clocks for 256 columns,
+// 500 for 192 and 440 for 128 (32, 28 and 24 KB per SM, at the 55 to 58 bytes per clock that L2
 // delivers to an SM: measured 566 and 444 on 4096 x 4096 x 11008), a tile 2500
 // more that nothing hides. One product: tiles beyond whole waves may be split;
 // then their parts fill waves of their own, and the partial tiles' way through L2
 // and a second launch come on top. Two products: all tiles of one or both may be
-// split, into parts of about the same length.
+// split, into parts of about the same length. 192 columns (forward only) are for
+// sizes that leave the last wave of wider tiles nearly empty: 12608 x 768 -> 768 in
+// float16 25.7 -> 22.3 us.
 static Schedule schedule_for(const Size* p, int count) {
   Schedule best{};
   best.clocks = 1e300;
-  for (int bn : {256, 128}) {
+  for (int bn : {256, 192, 128}) {
+    if (bn == 192 && (count == 2 || p[0].b_mn)) continue;  // B would come in boxes of 64 and 32
     Schedule s{};
     s.bn = bn;
     double block[2] = {0, 0};
@@ -944,7 +950,7 @@ static Schedule schedule_for(const Size* p, int count) {
       s.tiles_m[i] = (int)((p[i].m + 255) / 256);
       s.tiles_n[i] = (p[i].n + bn - 1) / bn;
       tiles[i] = (long long)s.tiles_m[i] * s.tiles_n[i];
-      block[i] = (bn == 256 ? 560.0 : 440.0) * p[i].segments;
+      block[i] = (bn == 256 ? 560.0 : bn == 192 ? 500.0 : 440.0) * p[i].segments;
     }
     auto part = [&](int i, int splits) { return ((p[i].kblocks + splits - 1) / splits) * block[i] + 2500.0; };
     auto joins = [&](int i, long long rest, int splits) { return splits > 1 ? (double)rest * (splits + 1) * 256 * bn * 4 / 2500.0 + 120.0 * splits : 0.0; };
@@ -1016,7 +1022,7 @@ struct Product {
   long long m, k;
   int n;
   Epilogue e;
-  Size size() const { return {m, n, (int)((k + KB - 1) / KB), plane_pairs(a.planes, b.planes)}; }
+  Size size() const { return {m, n, (int)((k + KB - 1) / KB), plane_pairs(a.planes, b.planes), b.mn}; }
 };
 
 template <class T, int BN, Kind KIND>
@@ -1085,6 +1091,9 @@ static cudaError_t launch_tc(const Product* products, int dtype, float* partial,
   }
   return with_dtype(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
+    if constexpr (KIND == Kind::forward) {
+      if (sc.bn == 192) return launch_tc_t<T, 192, KIND>(maps, args, items, rest, st);
+    }
     return sc.bn == 256 ? launch_tc_t<T, 256, KIND>(maps, args, items, rest, st) : launch_tc_t<T, 128, KIND>(maps, args, items, rest, st);
   });
 }
