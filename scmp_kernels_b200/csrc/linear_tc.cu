@@ -18,11 +18,12 @@
 //
 // Long sums (PROMOTE: every forward pass, and float32): the tensor core truncates
 // as it accumulates, a bias that grows with the length of the chain (1.4e-8
-// relative per 16 k values, measured); so a chain is cut every 1024 k values
+// relative per 16 k values, measured); so a chain is cut every 768 k values
 // (float32: 256), and the epilogue warps add the pieces in registers with
-// rounding while the MMAs fill the other accumulator. Cut every 1536 it gained
-// 2% on 4096 x 4096 x 8192 with GELU, and moved 1.6 times as many codes of the
-// checkpoint as a plain float32 sum does; cut every 1024, 1.3 times.
+// rounding while the MMAs fill the other accumulator. On 4096 x 4096 x 11008 with
+// GELU, chains of 512, 768, 1024 and 1536 move 0.93, 1.13, 1.32 and 1.6 times as
+// many codes of the checkpoint off the exact ones as a plain float32 sum does (in
+// the 2-norm); 512 takes 376 us, 768 359 us, 1024 347 us.
 //
 // The last wave, when its tiles do not fill the SMs: their k blocks are split
 // over several clusters, which leave float32 partial tiles that a second kernel
@@ -32,7 +33,7 @@
 // Measured (B200, back to back): 4096 x 4096 x 8192 bfloat16 180 us, 1.53
 // PFLOP/s or 0.93 of the measured cuBLAS rate (alone, at full clock, 152 to 176
 // us with the tensor pipe 88 to 92% busy; what remains is the first loads and the
-// last epilogue). With GELU and an 8-bit checkpoint 203 us: the epilogue of a
+// last epilogue). With GELU and an 8-bit checkpoint 210 us: the epilogue of a
 // tile (950 instructions a piece and warp) then outlasts the two accumulators
 // that the MMAs can fill meanwhile. Bound by the operands' way from L2 (58 bytes
 // per clock and SM against the 64 that 256 x 256 tiles want at full rate) and, in
@@ -1067,7 +1068,7 @@ static cudaError_t launch_tc(const Product* products, int dtype, float* partial,
       g.pa[s] = p.b.planes == 1 ? g.segments - 1 - s : p.a.planes == 1 ? 0 : six_a[s];
       g.pb[s] = p.a.planes == 1 ? g.segments - 1 - s : p.b.planes == 1 ? 0 : six_b[s];
     }
-    g.chunk = dtype == SCMP_F32 ? 4 : 16;
+    g.chunk = dtype == SCMP_F32 ? 4 : 12;
     g.tiles_m = sc.tiles_m[i];
     g.tiles_n = sc.tiles_n[i];
     g.whole = sc.whole[i];
